@@ -1,0 +1,63 @@
+// C ABI of the optimizer kernels in adamw.hip (host binding:
+// csrc/bind/adamw_binding.cpp).  dtype codes as in api.h.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+extern "C" {
+
+// One tensor of an AdamW step.  `w` is the float32 master, or the parameter
+// itself where that is float32 (then `p` is null).  `ms`/`vs` are the scales
+// of 8-bit moments, one a block of DDL_MOMENT_BLOCK elements; unused where
+// the moments are float32.
+struct DdlAdamTensor {
+  void* p;
+  const void* g;
+  float* w;
+  void* m;
+  void* v;
+  float* ms;
+  float* vs;
+  int64_t n;
+  float* step;     // the tensor's own step count, on the device
+  uint32_t index;  // its place in the optimizer: seeds the random rounding
+};
+
+struct DdlAdamScalars {
+  double lr, beta1, beta2, eps, weight_decay;
+  float grad_mul;   // 1 / grad_scale
+  uint32_t seed;
+};
+
+struct DdlGradTensor {
+  void* g;
+  int64_t n;
+};
+
+#define DDL_MOMENT_BLOCK 256
+
+// Step counts += 1, and the numbers that follow from them for each tensor.
+// ws: ddl_adamw_ws_bytes(count) bytes.
+int64_t ddl_adamw_ws_bytes(int64_t count);
+void ddl_adamw_prepare(const DdlAdamTensor* t, int64_t count,
+                       const DdlAdamScalars* c, void* ws, hipStream_t s);
+// The update of all tensors.  coef: device scalar that multiplies every
+// gradient (clipping), or null.
+void ddl_adamw(const DdlAdamTensor* t, int64_t count,
+               const DdlAdamScalars* c, int dtype, int bits, const void* ws,
+               const float* coef, hipStream_t s);
+
+// Global gradient norm.  partials: ddl_grad_norm_blocks() doubles for each
+// list, one after the other; ddl_grad_norm_finish folds `blocks` of them:
+// norm = sqrt(sum) * mul, coef = min(1, max_norm / (norm + 1e-6)).
+int64_t ddl_grad_norm_blocks(const DdlGradTensor* t, int64_t count);
+void ddl_grad_norm_partials(const DdlGradTensor* t, int64_t count, int dtype,
+                            double* partials, hipStream_t s);
+void ddl_grad_norm_finish(const double* partials, int64_t blocks, double mul,
+                          double max_norm, float* norm, float* coef,
+                          hipStream_t s);
+// g *= *coef; nothing is read or written where *coef is 1.
+void ddl_grad_scale(const DdlGradTensor* t, int64_t count, int dtype,
+                    const float* coef, hipStream_t s);
+
+}  // extern "C"

@@ -9,5 +9,5 @@ from .modules import (  # noqa: F401
     ReLU,
     cast_model_,
 )
-from .optim import FusedSGD  # noqa: F401
+from .optim import FusedAdamW, FusedSGD, clip_grad_norm_  # noqa: F401
 from ._ext import kernels_available, load_kernels_ext, load_comm_ext  # noqa: F401

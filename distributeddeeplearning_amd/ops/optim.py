@@ -1,4 +1,4 @@
-"""Fused optimizers (K10 SGD+momentum, K11 LARS).
+"""Fused optimizers (K10 SGD+momentum, K11 LARS, AdamW) and gradient clipping.
 
 The reference updates 161 ResNet-50 tensors with framework foreach kernels;
 here the whole model updates in ONE multi-tensor HIP kernel launch: a chunk
@@ -173,35 +173,446 @@ class FusedSGD(torch.optim.Optimizer):
         truncate the fp32 masters and momentum (and break the fused kernel,
         which reads them as 4-byte words).  Restore manually, moving device
         but never changing dtype."""
-        groups = self.param_groups
-        saved_groups = sd["param_groups"]
-        if len(groups) != len(saved_groups):
-            raise ValueError("loaded state dict has a different number of "
-                             "parameter groups")
-        id_map = {}
-        for g, sg in zip(groups, saved_groups):
-            if len(g["params"]) != len(sg["params"]):
-                raise ValueError("parameter group size mismatch in "
-                                 "load_state_dict")
-            for p, pid in zip(g["params"], sg["params"]):
-                id_map[pid] = p
-            for k, v in sg.items():
-                if k != "params":
-                    g[k] = v
-        self.state.clear()
-        for pid, st in sd["state"].items():
-            p = id_map.get(pid, pid)
-            dev = p.device if torch.is_tensor(p) else None
-            self.state[p] = {
-                k: (v.to(device=dev) if torch.is_tensor(v) and dev is not None
-                    else v)
-                for k, v in st.items()
-            }
+        _restore_exact(self, sd)
         self._tables = {}
 
     def invalidate_table(self):
         self._tables = {}
 
 
+def _restore_exact(opt, sd):
+    groups = opt.param_groups
+    saved_groups = sd["param_groups"]
+    if len(groups) != len(saved_groups):
+        raise ValueError("loaded state dict has a different number of "
+                         "parameter groups")
+    id_map = {}
+    for g, sg in zip(groups, saved_groups):
+        if len(g["params"]) != len(sg["params"]):
+            raise ValueError("parameter group size mismatch in "
+                             "load_state_dict")
+        for p, pid in zip(g["params"], sg["params"]):
+            id_map[pid] = p
+        for k, v in sg.items():
+            if k != "params":
+                g[k] = v
+    opt.state.clear()
+    for pid, st in sd["state"].items():
+        p = id_map.get(pid, pid)
+        dev = p.device if torch.is_tensor(p) else None
+        opt.state[p] = {
+            k: (v.to(device=dev) if torch.is_tensor(v) and dev is not None
+                else v)
+            for k, v in st.items()
+        }
+
+
 def _dtype_code(dt: torch.dtype) -> int:
     return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dt]
+
+
+# --------------------------------------------------------------------------
+# AdamW
+# --------------------------------------------------------------------------
+
+MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
+_E4M3_MAX = 448.0
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """The elements of a dense tensor in the order of its storage."""
+    return torch.as_strided(t.detach(), (t.numel(),), (1,),
+                            t.storage_offset())
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    need = 1
+    for stride, size in sorted((t.stride(d), t.size(d))
+                               for d in range(t.dim()) if t.size(d) > 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.shape == b.shape and all(
+        a.size(d) < 2 or a.stride(d) == b.stride(d) for d in range(a.dim()))
+
+
+def _mix32(x: torch.Tensor) -> torch.Tensor:
+    """The kernel's hash of 32 bits (held in int64)."""
+    x = x ^ (x >> 16)
+    x = (x * 0x6A09E667) & 0xFFFFFFFF
+    x = x ^ (x >> 15)
+    x = (x * 0x5DB3D743) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _blocks(x: torch.Tensor) -> torch.Tensor:
+    pad = -x.numel() % MOMENT_BLOCK
+    return torch.nn.functional.pad(x, (0, pad)).view(-1, MOMENT_BLOCK)
+
+
+def quantize_moment(x: torch.Tensor, r16: torch.Tensor):
+    """8-bit codes (uint8 bits of e4m3) and block scales of a flat float32
+    tensor.  A magnitude between two codes takes the upper one where the part
+    above the lower, in 2^-16 of their distance, plus ``r16`` (int64 in
+    [0, 2^16)) reaches 2^16.  Values that are not finite become NaN codes and
+    do not enter their block's scale; a block below 2^-100 becomes zeros."""
+    n = x.numel()
+    finite = torch.isfinite(x)
+    top = _blocks(torch.where(finite, x.abs(), 0.0)).amax(1)
+    tiny = top < 2.0 ** -100
+    scale = torch.where(tiny, 0.0, top * (1.0 / _E4M3_MAX))
+    inv = torch.where(tiny, 0.0, top.reciprocal() * _E4M3_MAX)
+    inv = inv.repeat_interleave(MOMENT_BLOCK)[:n]
+    y = torch.where(finite, x.abs() * inv, 0.0).clamp(max=_E4M3_MAX)
+    bits = (y.view(torch.int32).long() + (r16 << 4)) & ~0xFFFFF
+    normal = bits.int().view(torch.float32)
+    small = torch.floor(y * 512.0 + r16.float() * 2.0 ** -16) / 512.0
+    q = torch.where(y < 2.0 ** -6, small, normal)
+    q = torch.where(finite, torch.copysign(q, x), float("nan"))
+    return q.to(torch.float8_e4m3fn).view(torch.uint8), scale
+
+
+def dequantize_moment(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The float32 values of flat 8-bit codes."""
+    value = code.view(torch.float8_e4m3fn).float()
+    return value * scale.repeat_interleave(MOMENT_BLOCK)[:code.numel()]
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay), one fused pass over all tensors on GPU.
+
+    The mathematics is that of ``torch.optim.AdamW``::
+
+        w <- w - lr * weight_decay * w
+        m <- beta1 m + (1 - beta1) g,   v <- beta2 v + (1 - beta2) g^2
+        w <- w - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+
+    Parameters in bfloat16 or float16 have a float32 master that is updated
+    and then rounded; float32 parameters are their own master.
+
+    ``state_bits=8`` (also an option of a parameter group) holds ``m`` and
+    ``sqrt(v)`` as 8-bit e4m3 codes with one float32 scale for 256
+    consecutive elements: 2 bytes a parameter for both moments instead of 8.
+    Codes are rounded up or down by chance, so that they are right on
+    average; the chance is a hash of ``seed``, the step, the tensor and the
+    element, so that a run can be repeated bit for bit.
+
+    ``max_grad_norm`` clips the global norm of all gradients of the optimizer
+    (as ``clip_grad_norm_`` before the step would, without writing the
+    gradients); ``grad_norm`` then holds the norm of the last step.
+    ``grad_scale`` is the loss scale that the gradients still carry.
+
+    State tensors are updated in place; to replace them, load a state dict.
+    Step counts are held on the device, so a step captured into a graph
+    counts on at each replay, with the learning rate that it was captured
+    with.  Each parameter has to be dense in memory (channels_last is).
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+                 weight_decay=1e-2, state_bits=32, max_grad_norm=None,
+                 grad_scale=1.0, seed=0):
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps,
+                        weight_decay=weight_decay, state_bits=state_bits,
+                        seed=seed)
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be positive: {max_grad_norm}")
+        self._plans = None
+        super().__init__(params, defaults)
+        self.max_grad_norm = max_grad_norm
+        self.grad_scale = grad_scale  # multiply grads by 1/scale in the update
+        self.grad_norm = None
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        try:
+            self._check_group(group)
+        except (ValueError, TypeError):
+            self.param_groups.pop()
+            raise
+        self._plans = None
+
+    @staticmethod
+    def _check_group(group):
+        if not group["lr"] >= 0:
+            raise ValueError(f"invalid learning rate: {group['lr']}")
+        if len(group["betas"]) != 2 or not all(0 <= b < 1
+                                               for b in group["betas"]):
+            raise ValueError(f"betas lie in [0, 1): {group['betas']}")
+        if not group["eps"] >= 0:
+            raise ValueError(f"invalid eps: {group['eps']}")
+        if not group["weight_decay"] >= 0:
+            raise ValueError(f"invalid weight_decay: {group['weight_decay']}")
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32: {group['state_bits']}")
+        ids = [id(p) for p in group["params"]]
+        if len(set(ids)) != len(ids):
+            raise ValueError("a parameter appears twice in its group")
+        for p in group["params"]:
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                raise TypeError(f"parameters are float32, bfloat16 or "
+                                f"float16, not {p.dtype}")
+            if not _is_dense(p):
+                raise ValueError("a parameter is not dense in memory: the "
+                                 "update runs over its storage")
+
+    # ---- state ------------------------------------------------------------
+
+    def _init_state(self, p, bits):
+        st = self.state[p]
+        if "step" in st:
+            return st
+        st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+        if p.dtype != torch.float32:
+            st["master"] = p.detach().to(torch.float32)
+        kind = torch.uint8 if bits == 8 else torch.float32
+        for name in ("exp_avg", "exp_avg_sq"):
+            st[name] = torch.zeros_like(p, dtype=kind, requires_grad=False)
+            if bits == 8:
+                st[name + "_scale"] = torch.zeros(
+                    -(-p.numel() // MOMENT_BLOCK), dtype=torch.float32,
+                    device=p.device)
+        return st
+
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of a parameter as float32 tensors; copies
+        where they are held in 8 bits."""
+        st = self.state[p]
+        if "step" not in st:
+            raise KeyError("the parameter has no state yet")
+        if "exp_avg_scale" not in st:
+            return st["exp_avg"], st["exp_avg_sq"]
+        out = []
+        for name in ("exp_avg", "exp_avg_sq"):
+            value = torch.empty_like(p, dtype=torch.float32,
+                                     requires_grad=False)
+            _flat(value).copy_(dequantize_moment(_flat(st[name]),
+                                                 st[name + "_scale"]))
+            out.append(value)
+        return out[0], out[1].square_()
+
+    def refresh_master(self):
+        """Re-copy params into masters (after load_state_dict of the model
+        or broadcast_parameters)."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                if "master" in self.state.get(p, {}):
+                    self.state[p]["master"].copy_(p.detach())
+
+    def load_state_dict(self, sd):
+        """Exact-dtype restore, as FusedSGD's; the state tensors of ``sd``
+        are taken over without a copy where they are on the right device."""
+        _restore_exact(self, sd)
+        for group in self.param_groups:
+            group["betas"] = tuple(group["betas"])
+            for p in group["params"]:
+                self._adopt(p, self.state.get(p), group["state_bits"])
+        self._plans = None
+
+    @staticmethod
+    def _adopt(p, st, bits):
+        if not st:
+            return
+        if ("exp_avg_scale" in st) != (bits == 8):
+            raise ValueError("the loaded moments and the group's state_bits "
+                             "do not agree")
+        if p.dtype == torch.float32:
+            st.pop("master", None)
+        elif "master" not in st:
+            st["master"] = p.detach().to(torch.float32)
+        for name in ("master", "exp_avg", "exp_avg_sq"):
+            t = st.get(name)
+            if t is None or _same_layout(t, p):
+                continue
+            if t.shape != p.shape:
+                raise ValueError(f"{name} has another shape than its "
+                                 "parameter")
+            if bits == 8 and name != "master":
+                raise ValueError("8-bit moments belong to the memory layout "
+                                 "that they were saved in")
+            st[name] = torch.empty_like(p, dtype=t.dtype).copy_(t)
+        if not torch.is_tensor(st["step"]):
+            st["step"] = torch.tensor(float(st["step"]), device=p.device)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = None
+
+    def __getstate__(self):
+        state = super().__getstate__()
+        state.update(max_grad_norm=self.max_grad_norm,
+                     grad_scale=self.grad_scale, grad_norm=None, _plans=None)
+        return state
+
+    def invalidate_table(self):
+        """Nothing to do: gradients are looked up at every step."""
+
+    # ---- step -------------------------------------------------------------
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params = [p for g in self.param_groups for p in g["params"]]
+        if any(p.is_cuda for p in params):
+            self._step_gpu(params)
+        else:
+            self._step_cpu()
+        return loss
+
+    def _build_plans(self):
+        ext = load_kernels_ext()
+        self._plans = []
+        index = 0
+        for group in self.param_groups:
+            parts = {}
+            for p in group["params"]:
+                if not p.is_cuda:
+                    raise ValueError("parameters on the CPU and on a GPU in "
+                                     "one optimizer")
+                parts.setdefault((p.device, p.dtype), []).append((index, p))
+                index += 1
+            for members in parts.values():
+                states = [self.state.get(p, {}) for _, p in members]
+                columns = [[st.get(k) for st in states]
+                           for k in ("master", "exp_avg", "exp_avg_sq",
+                                     "exp_avg_scale", "exp_avg_sq_scale",
+                                     "step")]
+                plan = ext.AdamWPlan([p for _, p in members], *columns,
+                                     [i for i, _ in members],
+                                     group["state_bits"])
+                self._plans.append((plan, group, [p for _, p in members]))
+
+    def _step_gpu(self, params):
+        if self._plans is None:
+            self._build_plans()
+        missing = False
+        for plan, group, members in self._plans:
+            for i in plan.need():  # the first gradient of a parameter
+                self._init_state(members[i], group["state_bits"])
+                missing = True
+        if missing:
+            self._build_plans()
+        for plan, _, _ in self._plans:
+            plan.collect()
+        grad_mul = 1.0 / self.grad_scale
+        coef = None
+        if self.max_grad_norm is not None and self._plans:
+            ext = load_kernels_ext()
+            self.grad_norm, coef = ext.adamw_grad_norm(
+                [plan for plan, _, _ in self._plans], grad_mul,
+                float(self.max_grad_norm))
+        for plan, group, _ in self._plans:
+            beta1, beta2 = group["betas"]
+            plan.step(float(group["lr"]), float(beta1), float(beta2),
+                      float(group["eps"]), float(group["weight_decay"]),
+                      grad_mul, int(group["seed"]) & 0xFFFFFFFF, coef)
+
+    def _step_cpu(self):
+        mul = 1.0 / self.grad_scale
+        if self.max_grad_norm is not None:
+            grads = [p.grad for g in self.param_groups for p in g["params"]
+                     if p.grad is not None]
+            self.grad_norm, coef = _norm_cpu(grads, mul, self.max_grad_norm)
+            mul = mul * float(coef)
+        index = -1
+        for group in self.param_groups:
+            beta1, beta2 = group["betas"]
+            lr, bits = group["lr"], group["state_bits"]
+            for p in group["params"]:
+                index += 1
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("sparse gradients are not supported")
+                st = self._init_state(p, bits)
+                grad = p.grad.detach()
+                if not _same_layout(grad, p):
+                    grad = torch.empty_like(p).copy_(grad)
+                g = _flat(grad).to(torch.float32) * mul
+                w = _flat(st.get("master", p))
+                m, v = _flat(st["exp_avg"]), _flat(st["exp_avg_sq"])
+                st["step"] += 1
+                t = float(st["step"])
+                if bits == 8:
+                    codes = m, v
+                    m = dequantize_moment(m, st["exp_avg_scale"])
+                    v = dequantize_moment(v, st["exp_avg_sq_scale"])
+                    v = v * v
+                m_new = beta1 * m + (1.0 - beta1) * g
+                v_new = beta2 * v + (1.0 - beta2) * (g * g)
+                root = v_new.double().sqrt().float()  # correctly rounded
+                denom = root * (1.0 - beta2 ** t) ** -0.5 + group["eps"]
+                w.mul_(1.0 - lr * group["weight_decay"])
+                w.sub_((lr / (1.0 - beta1 ** t) * m_new) / denom)
+                if bits == 8:
+                    r = self._random_bits(group["seed"], index, int(t),
+                                          m.numel())
+                    for name, code, new, bits16 in (
+                            ("exp_avg", codes[0], m_new, r & 0xFFFF),
+                            ("exp_avg_sq", codes[1], root, r >> 16)):
+                        q, scale = quantize_moment(new, bits16)
+                        code.copy_(q)
+                        st[name + "_scale"].copy_(scale)
+                else:
+                    m.copy_(m_new)
+                    v.copy_(v_new)
+                if "master" in st:
+                    _flat(p).copy_(w)
+
+    @staticmethod
+    def _random_bits(seed, index, step, n):
+        stream = _mix32(torch.tensor(
+            (int(seed) + 0x9E3779B9 * (index + 1)) & 0xFFFFFFFF))
+        key = _mix32((stream + step) & 0xFFFFFFFF)
+        return _mix32((torch.arange(n) & 0xFFFFFFFF) ^ key)
+
+
+# --------------------------------------------------------------------------
+# Clipping of the global gradient norm
+# --------------------------------------------------------------------------
+
+def _norm_cpu(grads, mul, max_norm):
+    total = sum((g.detach().double().square().sum() for g in grads),
+                torch.zeros((), dtype=torch.float64))
+    norm = (total.sqrt() * mul).float()
+    return norm, (max_norm / (norm + 1e-6)).clamp(max=1.0)
+
+
+@torch.no_grad()
+def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
+    """Scale all gradients in place so that their global 2-norm is at most
+    ``max_norm``; returns the norm before (0-dim float32, no host sync).
+
+    ``grad_scale`` is the loss scale that the gradients carry: the norm, and
+    the bound, are of the gradients divided by it, and they keep carrying it.
+    As in ``torch.nn.utils.clip_grad_norm_``, a norm that is not finite is
+    not caught: it makes the gradients zero or NaN.
+
+    Under data parallelism call it after ``DistributedOptimizer.synchronize``;
+    every rank then computes the same norm.  Two launches read and fold, a
+    third scales; gradients are not touched where the norm is within bounds.
+    """
+    params = [params] if torch.is_tensor(params) else list(params)
+    if not max_norm > 0:
+        raise ValueError(f"max_norm must be positive: {max_norm}")
+    if not grad_scale > 0:
+        raise ValueError(f"grad_scale must be positive: {grad_scale}")
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        device = params[0].device if params else None
+        return torch.zeros((), dtype=torch.float32, device=device)
+    if grads[0].is_cuda:
+        return load_kernels_ext().clip_grads(grads, 1.0 / grad_scale,
+                                             float(max_norm))
+    norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
+    if not float(coef) == 1.0:
+        for g in grads:
+            g.copy_(g.float() * coef)
+    return norm

@@ -36,6 +36,9 @@ HIPCC_FLAGS = [
     # this target (the host pass warns that it does not know the feature)
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+# Kernels that keep IEEE meaning (infinities and NaN in inputs, correctly
+# rounded division and roots) are compiled without fast-math.
+IEEE_KERNELS = {"adamw", "linear"}
 
 
 def compile_hip_objects() -> list:
@@ -55,7 +58,9 @@ def compile_hip_objects() -> list:
 
     def run(job):
         src, obj = job
-        cmd = [HIPCC, *HIPCC_FLAGS, "-c", str(src), "-o", str(obj)]
+        flags = [f for f in HIPCC_FLAGS
+                 if f != "-ffast-math" or src.stem not in IEEE_KERNELS]
+        cmd = [HIPCC, *flags, "-c", str(src), "-o", str(obj)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
@@ -80,7 +85,7 @@ common = dict(
 ext_modules = [
     CppExtension(
         "distributeddeeplearning_amd._C_kernels",
-        ["csrc/bind/kernels_binding.cpp"],
+        ["csrc/bind/kernels_binding.cpp", "csrc/bind/adamw_binding.cpp"],
         extra_objects=kernel_objs,
         libraries=["amdhip64"],
         **common,
