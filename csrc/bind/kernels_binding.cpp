@@ -643,9 +643,11 @@ void lars_norms(at::Tensor table, at::Tensor norms, int64_t dtype, double wd,
 }  // namespace
 
 void bind_adamw(pybind11::module& m);
+void bind_linear(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_adamw(m);
+  bind_linear(m);
   m.def("conv_fwd", &conv_fwd);
   m.def("conv_fwd_stats", &conv_fwd_stats);
   m.def("conv_dgrad", &conv_dgrad);

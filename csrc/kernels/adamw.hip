@@ -426,6 +426,7 @@ __global__ __launch_bounds__(THREADS) void grad_scale_k(
 // ---- host ------------------------------------------------------------------
 
 constexpr int CHUNK = 8192;
+constexpr int64_t MAX_BLOCKS = 1 << 23;  // a grid holds below 2^32 threads
 static_assert(CHUNK % MOMENT_BLOCK == 0, "a chunk holds whole blocks");
 
 bool takes16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -446,7 +447,7 @@ void in_groups(int64_t count, Size size, Fill fill, Launch launch) {
   };
   for (int64_t i = 0; i < count; ++i) {
     const int64_t more = cdiv(size(i), CHUNK);
-    if (a.count == MAX || blocks + more > (1 << 30)) flush(i);
+    if (a.count == MAX || blocks + more > MAX_BLOCKS) flush(i);
     fill(a, a.count, i);
     a.first[a.count++] = (int)blocks;
     blocks += more;

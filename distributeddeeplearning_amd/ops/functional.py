@@ -16,10 +16,12 @@ from __future__ import annotations
 
 from typing import Optional
 
+import math
 import os
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ._ext import load_kernels_ext
 
@@ -430,6 +432,103 @@ def global_avg_pool(x):
 
 def linear(x, weight, bias=None):
     return F.linear(x, weight, bias)
+
+
+# --------------------------------------------------------------------------
+# Dense layer with activation and residual in the product's epilogue
+# --------------------------------------------------------------------------
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_DENSE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _LinearActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        ext = load_kernels_ext()
+        # ReLU's output tells where its input was positive; with a residual
+        # on top, and for the smooth activations, the input itself is kept
+        by_output = act == ACTIVATIONS["relu"] and residual is None
+        want_z = act != 0 and not by_output and any(ctx.needs_input_grad[:3])
+        y, z = ext.linear_fwd(x, weight, bias, residual, act, want_z)
+        ctx.act = act
+        kept = y if by_output else z if want_z else None
+        ctx.save_for_backward(x, weight, kept)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ext = load_kernels_ext()
+        x, weight, kept = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            dx, dw, db = ext.linear_bwd(dy, x, weight, kept, ctx.act, need_x,
+                                        need_w, need_b)
+        return dx, dw, db, dy if need_r else None, None
+
+
+def _cpu_activation(z, activation):
+    if activation == "relu":
+        return F.relu(z)
+    if activation == "gelu":
+        return F.gelu(z)
+    if activation == "gelu_tanh":
+        return F.gelu(z, approximate="tanh")
+    if activation == "silu":
+        return F.silu(z)
+    return z
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """``activation(x @ weight.T + bias) + residual`` in one product.
+
+    ``x``: (..., in), ``weight``: (out, in), ``bias``: (out,), ``residual``:
+    anything that broadcasts to (..., out); all float32, bfloat16 or float16
+    alike.  ``activation``: "none", "relu", "gelu" (erf), "gelu_tanh" or
+    "silu".  Sums, bias, activation and residual are computed in float32 and
+    rounded once.  Differentiable once in every tensor; the backward pass
+    rounds the activation's gradient to the inputs' dtype before its products.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, not "
+                         f"{activation!r}")
+    if weight.dim() != 2:
+        raise ValueError(f"weight has shape (out, in), not {tuple(weight.shape)}")
+    out, inp = weight.shape
+    if x.dim() < 1 or x.shape[-1] != inp:
+        raise ValueError(f"x ends in {inp} features, its shape is "
+                         f"{tuple(x.shape)}")
+    if bias is not None and tuple(bias.shape) != (out,):
+        raise ValueError(f"bias has shape ({out},), not {tuple(bias.shape)}")
+    if x.dtype not in _DENSE_DTYPES:
+        raise TypeError(f"x is float32, bfloat16 or float16, not {x.dtype}")
+    for name, t in (("weight", weight), ("bias", bias),
+                    ("residual", residual)):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise TypeError(f"{name} is {t.dtype} on {t.device}, x is "
+                            f"{x.dtype} on {x.device}")
+    shape = x.shape[:-1] + (out,)
+    if residual is not None:
+        try:
+            residual = residual.broadcast_to(shape)
+        except RuntimeError as e:
+            raise ValueError(f"residual of shape {tuple(residual.shape)} does "
+                             f"not broadcast to {tuple(shape)}") from e
+    if not x.is_cuda:
+        z = F.linear(x.float(), weight.float(),
+                     None if bias is None else bias.float())
+        y = _cpu_activation(z, activation)
+        if residual is not None:
+            y = y + residual.float()
+        return y.to(x.dtype)
+    rows = math.prod(shape[:-1])
+    y = _LinearActFn.apply(
+        x.reshape(rows, inp), weight, bias,
+        None if residual is None else residual.reshape(rows, out),
+        ACTIVATIONS[activation])
+    return y.view(shape)
 
 
 # --------------------------------------------------------------------------

@@ -159,8 +159,18 @@ class GlobalAvgPool2d(nn.Module):
 
 
 class Linear(nn.Module):
-    def __init__(self, in_features, out_features, bias=True):
+    """Dense layer.  With an ``activation`` ("relu", "gelu", "gelu_tanh",
+    "silu"), or a ``residual`` at call time, they are applied in the product's
+    epilogue (``functional.linear_act``); without either this is a plain
+    library product."""
+
+    def __init__(self, in_features, out_features, bias=True,
+                 activation="none"):
         super().__init__()
+        if activation not in DF.ACTIVATIONS:
+            raise ValueError(f"activation is one of {sorted(DF.ACTIVATIONS)}, "
+                             f"not {activation!r}")
+        self.activation = activation
         self.in_features = in_features
         self.out_features = out_features
         self.weight = nn.Parameter(torch.empty(out_features, in_features))
@@ -175,11 +185,17 @@ class Linear(nn.Module):
         if self.bias is not None:
             nn.init.zeros_(self.bias)
 
-    def forward(self, x):
-        return DF.linear(x, self.weight, self.bias)
+    def forward(self, x, residual: Optional[torch.Tensor] = None):
+        if self.activation == "none" and residual is None:
+            return DF.linear(x, self.weight, self.bias)
+        return DF.linear_act(x, self.weight, self.bias, self.activation,
+                             residual)
 
     def extra_repr(self):
-        return f"in_features={self.in_features}, out_features={self.out_features}"
+        act = ("" if self.activation == "none"
+               else f", activation={self.activation}")
+        return (f"in_features={self.in_features}, "
+                f"out_features={self.out_features}{act}")
 
 
 class Dropout(nn.Module):

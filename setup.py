@@ -85,7 +85,8 @@ common = dict(
 ext_modules = [
     CppExtension(
         "distributeddeeplearning_amd._C_kernels",
-        ["csrc/bind/kernels_binding.cpp", "csrc/bind/adamw_binding.cpp"],
+        ["csrc/bind/kernels_binding.cpp", "csrc/bind/adamw_binding.cpp",
+         "csrc/bind/linear_binding.cpp"],
         extra_objects=kernel_objs,
         libraries=["amdhip64"],
         **common,

@@ -1,0 +1,426 @@
+"""functional.linear_act, forward and backward, against the formulas in 64
+bits, on the CPU and on the GPU.
+
+Bounds, element by element.  U is half a step of float32, H half a step of
+the inputs' dtype.  A sum of K products in float32 misses by at most
+(K + 1) U times the sum of the products' magnitudes, whatever its order.
+The activations have slopes below 1.13 and are evaluated to 16 U of |z| + 1
+(exp and erf are good to a few steps); their second derivatives are below 1.
+The backward pass takes z rounded to the dtype and rounds dz to it, then sums
+as the forward does.  Where |z| is within its own error of ReLU's corner, the
+gradient may be either side's.
+"""
+import pytest
+import torch
+
+from distributeddeeplearning_amd import ops
+from distributeddeeplearning_amd.ops import functional as DF
+
+U = torch.finfo(torch.float32).eps / 2
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2 if dtype != torch.float32 else U
+
+
+def floor(dtype):
+    """Half the distance of the dtype's smallest numbers."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def act64(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "gelu":
+        return z * torch.special.ndtr(z)
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh((2 / torch.pi) ** 0.5
+                                         * (z + 0.044715 * z ** 3)))
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return z * 1.0
+
+
+def check(got, want, room):
+    off = (got.detach().cpu().double() - want).abs()
+    assert got.shape == want.shape
+    worst = (off - room).max() if off.numel() else torch.tensor(0.0)
+    assert (off <= room).all(), float(worst)
+
+
+def run_case(m, k, n, dtype, device, act, bias=True, residual=True,
+             change=lambda t: t, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+
+    def rand(*shape, std=1.0):
+        return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+    host = {"x": rand(m, k), "w": rand(n, k, std=(2 / max(k, 1)) ** 0.5)}
+    if bias:
+        host["b"] = rand(n, std=0.3)
+    if residual:
+        host["r"] = rand(m, n)
+    dy = rand(m, n)
+    leaf = {key: change(t.to(device)).requires_grad_(True)
+            for key, t in host.items()}
+    y = DF.linear_act(leaf["x"], leaf["w"], leaf.get("b"), act,
+                      leaf.get("r"))
+    assert y.dtype == dtype and y.shape == (m, n) and y.is_contiguous()
+    y.backward(change(dy.to(device)))
+
+    h, f = half(dtype), floor(dtype)
+    d = {key: t.double() for key, t in host.items()}
+    zero = torch.zeros((), dtype=torch.float64)
+    z = d["x"] @ d["w"].t() + d.get("b", zero)
+    ez = (k + 2) * U * (d["x"].abs() @ d["w"].abs().t()
+                        + d.get("b", zero).abs())
+    z.requires_grad_(True)
+    a = act64(z, act)
+    (slope,) = torch.autograd.grad(a, z, torch.ones_like(z))
+    z, a = z.detach(), a.detach()
+    want = a + d.get("r", zero)
+    ey = 1.13 * ez + 16 * U * (z.abs() + 1) + 2 * U * want.abs()
+    check(y, want, ey + h * (want.abs() + ey) + f)
+
+    g = dy.double()
+    dz = g * slope
+    if act == "none":
+        edz = zero * dz
+    elif act == "relu":
+        edz = torch.where(z.abs() <= ez + f, g.abs(), zero)
+    else:
+        edz = g.abs() * (ez + h * z.abs() + 16 * U * (z.abs() + 2))
+    edb = edz + 2 * U * dz.abs()
+    if act != "none":
+        edz = edz + h * (dz.abs() + edz) + f
+    ax, aw = d["x"].abs(), d["w"].abs()
+    big = dz.abs() + edz
+
+    def bound(err, size, terms, ref):
+        e = err + (terms + 1) * U * size
+        return e + h * (ref.abs() + e) + f
+
+    dx, dw = dz @ d["w"], dz.t() @ d["x"]
+    check(leaf["x"].grad, dx, bound(edz @ aw, big @ aw, n, dx))
+    check(leaf["w"].grad, dw, bound(edz.t() @ ax, big.t() @ ax, m, dw))
+    if bias:
+        db = dz.sum(0)
+        check(leaf["b"].grad, db, bound(edb.sum(0), big.sum(0), m, db))
+    if residual:
+        assert torch.equal(leaf["r"].grad.cpu(), dy)
+
+
+SHAPES = [(1, 1, 1), (1, 8, 8), (2, 64, 16), (3, 5, 7), (16, 256, 40),
+          (17, 72, 130), (33, 9, 1000), (63, 129, 257), (129, 128, 128),
+          (130, 66, 255), (256, 2048, 24), (257, 520, 264), (512, 40, 513)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_shapes(shape, dtype, device):
+    act = ACTS[(shape[0] + shape[1]) % 5]
+    run_case(*shape, dtype, device, act)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias,residual", [(True, True), (True, False),
+                                           (False, True), (False, False)])
+def test_epilogues(act, bias, residual, dtype, device):
+    run_case(70, 96, 136, dtype, device, act, bias, residual)
+    run_case(5, 31, 21, dtype, device, act, bias, residual)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(300, 4096, 500), (1000, 1000, 1003),
+                                   (2050, 2056, 770), (16, 9000, 640),
+                                   (1, 25088, 1000), (700, 30, 3000)])
+def test_larger(shape, dtype):
+    run_case(*shape, dtype, "cuda", "gelu" if shape[0] % 2 else "relu")
+
+
+def _offset(t):
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return flat[1:].view(t.shape).copy_(t)
+
+
+def _transposed(t):
+    return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+
+def _sliced(t):
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 24, dtype=t.dtype,
+                       device=t.device)
+    wide[..., 16:-8] = t
+    return wide[..., 16:-8]
+
+
+def _odd_rows(t):
+    wide = torch.full((*t.shape[:-1], t.shape[-1] + 3), float("nan"),
+                      dtype=t.dtype, device=t.device)
+    wide[..., :-3] = t
+    return wide[..., :-3]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", [_offset, _transposed, _sliced, _odd_rows])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(40, 64, 72), (1, 64, 72), (13, 15, 17)])
+def test_layouts(shape, dtype, change, device):
+    run_case(*shape, dtype, device, "silu",
+             change=lambda t: change(t.detach()).detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_lies_beyond_is_not_read(device):
+    """NaN around every operand leaves no trace."""
+    def change(t):
+        wide = torch.full((t.shape[0] + 8,) + tuple(
+            s + 16 for s in t.shape[1:]), float("nan"), dtype=t.dtype,
+            device=t.device)
+        view = wide[4:-4] if t.dim() == 1 else wide[4:-4, 8:-8]
+        return view.copy_(t).detach()
+    for shape in ((130, 72, 136), (1, 24, 8), (12, 72, 40), (129, 8, 129)):
+        run_case(*shape, torch.bfloat16, device, "gelu", change=change)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("m,k,n", [(0, 4, 5), (3, 0, 5), (3, 4, 0)])
+def test_empty(m, k, n, device):
+    x = torch.randn(m, k, device=device, requires_grad=True)
+    w = torch.randn(n, k, device=device, requires_grad=True)
+    b = torch.randn(n, device=device, requires_grad=True)
+    y = DF.linear_act(x, w, b, "relu")
+    assert y.shape == (m, n)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and (x.grad == 0).all()
+    assert w.grad.shape == w.shape and (w.grad == 0).all()
+    if k == 0:
+        assert torch.equal(y.detach(), b.detach().relu().expand(3, 5))
+        assert torch.equal(b.grad, 3.0 * (b.detach() > 0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_leading_dimensions_and_broadcast_residual(device):
+    torch.manual_seed(0)
+    x = torch.randn(2, 3, 4, 8, device=device, requires_grad=True)
+    w = torch.randn(16, 8, device=device, requires_grad=True)
+    r = torch.randn(3, 1, 16, device=device, requires_grad=True)
+    y = DF.linear_act(x, w, None, "silu", r)
+    assert y.shape == (2, 3, 4, 16)
+    dy = torch.randn_like(y)
+    y.backward(dy)
+    want = torch.nn.functional.silu(x.detach().double()
+                                    @ w.detach().double().t()) + r.double()
+    assert (y.double() - want).abs().max() < 64 * U * 10
+    assert (r.grad.double() - dy.double().sum((0, 2), keepdim=True)[0]
+            ).abs().max() < 16 * U * 8
+    one = DF.linear_act(x.detach()[0, 0, 0], w.detach())
+    assert one.shape == (16,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_only_the_gradients_asked_for(device):
+    x = torch.randn(9, 16, device=device)
+    w = torch.randn(8, 16, device=device, requires_grad=True)
+    b = torch.randn(8, device=device)
+    DF.linear_act(x, w, b, "gelu").sum().backward()
+    assert x.grad is None and b.grad is None and w.grad is not None
+    x.requires_grad_(True)
+    r = torch.zeros(9, 8, device=device, requires_grad=True)
+    y = DF.linear_act(x, w.detach(), b, "relu", r)
+    gx, gr = torch.autograd.grad(y.sum(), (x, r))
+    assert gx.shape == x.shape and (gr == 1).all()
+    y = DF.linear_act(x.detach(), w.detach(), b, "relu", r)
+    (gr,) = torch.autograd.grad(y.sum(), (r,))
+    assert (gr == 1).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_gradient_against_differences(act, device):
+    """Along one direction: (f(t) - f(-t)) / 2t misses the derivative by
+    t^2 / 6 of the third derivative (below 4 per unit of z' cubed for these
+    activations) and by float32's error of f over t."""
+    torch.manual_seed(1)
+    m, k, n, t = 6, 40, 24, 1e-2
+    x = torch.randn(m, k, device=device)
+    w = (torch.randn(n, k, device=device) / k ** 0.5).requires_grad_(True)
+    b = torch.randn(n, device=device)
+    direction = torch.randn(n, k, device=device) / k ** 0.5
+    dy = torch.randn(m, n, device=device)
+    DF.linear_act(x, w, b, act).backward(dy)
+    along = float((w.grad.double() * direction.double()).sum())
+    with torch.no_grad():
+        up, down = (DF.linear_act(x, w + s * direction, b, act).double()
+                    for s in (t, -t))
+    difference = float(((up - down) * dy.double()).sum()) / (2 * t)
+    slope = (x.double() @ direction.double().t()).abs()
+    room = float((dy.double().abs() * (4 / 6 * t * t * slope ** 3
+                                       + (k + 20) * U * 8 / t)).sum())
+    assert abs(along - difference) < room
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_that_are_not_finite_stay_in_their_row(device, dtype):
+    torch.manual_seed(0)
+    m, k, n = 150, 64, 130
+    x = torch.randn(m, k).to(device, dtype)
+    w = (torch.rand(n, k) + 0.1).to(device, dtype)
+    clean = DF.linear_act(x, w, None, "relu")
+    x[3, 5] = float("inf")
+    x[140, 63] = float("nan")
+    x[20, 0] = -float("inf")
+    y = DF.linear_act(x, w, None, "relu")
+    assert (y[3] == float("inf")).all()
+    assert torch.isnan(y[140]).all()
+    assert (y[20] == 0).all()
+    keep = [i for i in range(m) if i not in (3, 20, 140)]
+    assert torch.equal(y[keep], clean[keep])
+
+
+@gpu
+def test_offsets_past_32_bits():
+    n = (1 << 25) + 8  # 2^31 elements and some, 4 GiB
+    w = torch.zeros(n, 64, dtype=torch.bfloat16, device="cuda")
+    w[-3:] = 1.0
+    x = torch.ones(2, 64, dtype=torch.bfloat16, device="cuda")
+    y = DF.linear_act(x, w)
+    assert (y[:, -3:] == 64).all() and int((y != 0).sum()) == 6
+    del w
+    x = torch.zeros(n, 64, dtype=torch.bfloat16, device="cuda")
+    x[-2:] = 1.0
+    w = torch.ones(8, 64, dtype=torch.bfloat16, device="cuda")
+    w.requires_grad_(True)
+    y = DF.linear_act(x, w)
+    assert (y[-2:] == 64).all() and int((y != 0).sum()) == 16
+    y.backward(torch.ones_like(y))
+    assert (w.grad == 2).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_twice_is_bit_equal(dtype):
+    torch.manual_seed(0)
+    x = torch.randn(200, 5000, device="cuda").to(dtype)
+    w = torch.randn(300, 5000, device="cuda").to(dtype).requires_grad_(True)
+    b = torch.randn(300, device="cuda").to(dtype).requires_grad_(True)
+    runs = []
+    for _ in range(2):
+        y = DF.linear_act(x, w, b, "gelu")
+        runs.append((y, *torch.autograd.grad(y, (w, b), torch.ones_like(y))))
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+@gpu
+def test_another_stream():
+    torch.manual_seed(0)
+    x = torch.randn(300, 4096, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(500, 4096, device="cuda", dtype=torch.bfloat16)
+    want = DF.linear_act(x, w, None, "silu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = DF.linear_act(x, w, None, "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(want, got)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(4, 2000, 300), (200, 4099, 301)])
+def test_captured_forward_and_backward(shape):
+    m, k, n = shape
+    torch.manual_seed(0)
+    x, w, b = (torch.randn(s, device="cuda", dtype=torch.bfloat16)
+               for s in ((m, k), (n, k), (n,)))
+    dy = torch.randn(m, n, device="cuda", dtype=torch.bfloat16)
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = DF.linear_act(*leaves, "gelu")
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for k_ in range(4):
+        x.mul_(0.5).add_(0.01 * k_)
+        dy.neg_()
+        want = step()
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(want, out))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_module(device):
+    torch.manual_seed(0)
+    layer = ops.Linear(24, 16, activation="gelu").to(device)
+    x = torch.randn(5, 24, device=device)
+    r = torch.randn(5, 16, device=device)
+    want = torch.nn.functional.gelu(torch.nn.functional.linear(
+        x, layer.weight, layer.bias)) + r
+    # 24 products of at most 5 by 0.1, and the activation
+    assert (layer(x, r) - want).abs().max() < 64 * U * 12
+    assert "gelu" in repr(layer)
+    plain = ops.Linear(24, 16).to(device)
+    assert torch.equal(plain(x), torch.nn.functional.linear(
+        x, plain.weight, plain.bias))
+    with pytest.raises(ValueError, match="activation"):
+        ops.Linear(4, 4, activation="tanh")
+
+
+def test_refused_arguments():
+    x, w, b = torch.randn(3, 8), torch.randn(5, 8), torch.randn(5)
+    with pytest.raises(ValueError, match="activation"):
+        DF.linear_act(x, w, b, "swish")
+    with pytest.raises(ValueError, match="features"):
+        DF.linear_act(x[:, :7], w, b)
+    with pytest.raises(ValueError, match="features"):
+        DF.linear_act(torch.tensor(1.0), w, b)
+    with pytest.raises(ValueError, match="weight"):
+        DF.linear_act(x, w[0], b)
+    with pytest.raises(ValueError, match="bias"):
+        DF.linear_act(x, w, b[:4])
+    with pytest.raises(ValueError, match="broadcast"):
+        DF.linear_act(x, w, b, "none", torch.randn(2, 5))
+    with pytest.raises(ValueError, match="broadcast"):
+        DF.linear_act(x, w, b, "none", torch.randn(2, 3, 5))
+    with pytest.raises(TypeError, match="weight"):
+        DF.linear_act(x, w.double(), b)
+    with pytest.raises(TypeError, match="x is"):
+        DF.linear_act(x.double(), w.double())
+    with pytest.raises(TypeError, match="residual"):
+        DF.linear_act(x, w, b, "none", torch.randn(3, 5).half())
+
+
+@gpu
+def test_refused_on_the_gpu():
+    x = torch.randn(3, 8, device="cuda")
+    w = torch.randn(5, 8, device="cuda", requires_grad=True)
+    with pytest.raises(TypeError, match="cpu"):
+        DF.linear_act(x, w.cpu())
+    y = DF.linear_act(x, w, None, "silu")
+    (g,) = torch.autograd.grad(y.sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
