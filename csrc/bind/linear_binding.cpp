@@ -1,16 +1,21 @@
-// Torch binding of the dense layer (csrc/kernels/linear.hip): checks, packs
+// Torch binding of the dense layer (csrc/kernels/linear*.hip): checks, packs
 // operands whose rows do not lie on 16-byte boundaries, allocates outputs and
-// workspaces, and launches on the current stream of the tensors' device.
+// workspaces, and launches on the current stream of the tensors' device.  The
+// autograd function is here too: in Python it would cost a small layer more
+// time than its kernels.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "kernels/linear_api.h"
 
 namespace {
 
 using Maybe = c10::optional<at::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 hipStream_t stream_now() {
   return c10::hip::getCurrentHIPStream().stream();
@@ -22,27 +27,15 @@ int code_of(at::ScalarType t) {
     case at::kBFloat16: return 1;
     case at::kHalf: return 2;
     default:
-      TORCH_CHECK(false, "expected float32, bfloat16 or float16, got ", t);
+      TORCH_CHECK_TYPE(false, "x is float32, bfloat16 or float16, not ", t);
   }
-}
-
-void check_like(const at::Tensor& t, const at::Tensor& x, const char* name) {
-  TORCH_CHECK(t.device() == x.device(), name, " is on another device than x");
-  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name,
-              " has another dtype than x");
-}
-
-void check_matrix(const at::Tensor& t, int64_t rows, int64_t cols,
-                  const char* name) {
-  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name,
-              " has shape ", t.sizes(), ", expected (", rows, ", ", cols, ")");
 }
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // A matrix whose columns are neighbours in memory; its rows may lie anywhere.
 at::Tensor inner_contiguous(const at::Tensor& t) {
-  return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
+  return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
 }
 
 // Elements from one row to the next; a single row has no say.
@@ -50,30 +43,39 @@ int64_t row_stride(const at::Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
-// What the kernel reads: rows that begin and end at 16 bytes, no further
-// apart than its 32-bit offsets inside a tile reach.
-struct Operand {
-  at::Tensor keep;
-  const void* data;
-  int64_t ld;
-};
+// Rows that the tiled kernel reads as they are: they begin and end at 16
+// bytes, and are no further apart than its 32-bit offsets inside a tile reach.
+int64_t reach(const at::Tensor& t) {
+  return ((int64_t)1 << 31) / 256 / t.element_size();
+}
 
-Operand operand(const at::Tensor& matrix) {
-  const at::Tensor t = inner_contiguous(matrix);
+bool fits(const at::Tensor& t) {
   const int64_t per = 16 / t.element_size();
-  const int64_t reach = ((int64_t)1 << 31) / 256 / t.element_size();
-  const int64_t ld = row_stride(t);
-  if (ld % per == 0 && t.size(1) % per == 0 && ld < reach &&
-      ((uintptr_t)t.const_data_ptr() & 15) == 0)
-    return {t, t.const_data_ptr(), ld};
-  const int64_t wide = round_up(t.size(1), per);
-  TORCH_CHECK(wide < reach, "a matrix has ", t.size(1),
-              " columns, more than the kernel's offsets reach (", reach, ")");
-  at::Tensor packed = at::empty({t.size(0), wide}, t.options());
-  if (packed.numel())
-    ddl_pack_rows(t.const_data_ptr(), ld, packed.data_ptr(), wide, t.size(0),
-                  t.size(1), code_of(t.scalar_type()), stream_now());
-  return {packed, packed.const_data_ptr(), wide};
+  return (t.size(1) <= 1 || t.stride(1) == 1) && row_stride(t) % per == 0 &&
+         t.size(1) % per == 0 && row_stride(t) < reach(t) &&
+         ((uintptr_t)t.const_data_ptr() & 15) == 0;
+}
+
+// The same matrices with rows padded by zeros to 16 bytes where they do not
+// fit, in one launch.
+void pack(at::Tensor* a, at::Tensor* b) {
+  DdlPack todo[2];
+  at::Tensor from[2];
+  int count = 0, dtype = 0;
+  for (at::Tensor* t : {a, b}) {
+    if (t == nullptr || fits(*t)) continue;
+    from[count] = inner_contiguous(*t);
+    const at::Tensor& src = from[count];
+    const int64_t wide = round_up(src.size(1), 8);
+    TORCH_CHECK(wide < reach(src), "a matrix has ", src.size(1),
+                " columns, the kernel's offsets reach ", reach(src));
+    at::Tensor dst = at::empty({src.size(0), wide}, src.options());
+    todo[count++] = DdlPack{src.const_data_ptr(), dst.data_ptr(),
+                            row_stride(src), wide, src.size(0), src.size(1)};
+    dtype = code_of(src.scalar_type());
+    *t = dst;
+  }
+  if (count) ddl_pack_rows(todo, count, dtype, stream_now());
 }
 
 // out = epilogue(a b^T) with its workspace.
@@ -85,146 +87,258 @@ void product(DdlProduct& p, const at::Tensor& like) {
     p.slabs = slabs.data_ptr<float>();
   }
   ddl_product(&p, stream_now());
-  C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-// y = act(x w^T + bias) + residual, and z = x w^T + bias if asked for.
-std::tuple<at::Tensor, at::Tensor> linear_fwd(at::Tensor x, at::Tensor w,
-                                              Maybe bias, Maybe residual,
-                                              int64_t act, bool want_z) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2,
-              "x and weight are matrices on a GPU");
-  TORCH_CHECK(act >= 0 && act <= 4, "unknown activation ", act);
-  const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
-  const int dtype = code_of(x.scalar_type());
-  check_like(w, x, "weight");
-  check_matrix(w, n, k, "weight");
+// y = act(x w^T + bias) + residual, and z = x w^T + bias if asked for.  x and
+// w are replaced by what the kernel read.
+at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
+                      const Maybe& residual, int64_t act, at::Tensor* z) {
   c10::DeviceGuard guard(x.device());
+  const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
   at::Tensor y = at::empty({m, n}, x.options());
-  at::Tensor z = want_z ? at::empty({m, n}, x.options()) : at::Tensor();
   at::Tensor b, res;
   DdlProduct p{};
-  if (bias.has_value()) {
-    check_like(*bias, x, "bias");
-    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == n, "bias has shape ",
-                bias->sizes(), ", expected (", n, ")");
-    b = bias->contiguous();
-    p.bias = b.const_data_ptr();
-  }
-  if (residual.has_value()) {
-    check_like(*residual, x, "residual");
-    check_matrix(*residual, m, n, "residual");
-    res = inner_contiguous(*residual);
-    p.residual = res.const_data_ptr();
-    p.ldres = row_stride(res);
-  }
-  const Operand a = operand(x), c = operand(w);
-  p.a = a.data;
-  p.lda = a.ld;
-  p.b = c.data;
-  p.ldb = c.ld;
+  p.dtype = code_of(x.scalar_type());
+  p.act = (int)act;
   p.m = m;
   p.n = n;
   p.r = k;
   p.out = y.data_ptr();
   p.ldo = n;
-  p.z = want_z ? z.data_ptr() : nullptr;
-  p.act = (int)act;
-  p.dtype = dtype;
-  product(p, x);
-  return {y, z};
+  if (z) {
+    // float32: z rounded to 16 bits would cost the gradients a third rounding
+    // beside dz's and their own
+    *z = at::empty({m, n}, x.options().dtype(at::kFloat));
+    p.z = z->data_ptr<float>();
+  }
+  if (bias.has_value()) {
+    b = bias->contiguous();
+    p.bias = b.const_data_ptr();
+  }
+  if (residual.has_value()) {
+    res = inner_contiguous(*residual);
+    p.residual = res.const_data_ptr();
+    p.ldres = row_stride(res);
+  }
+  if (m == 0 || n == 0) return y;
+  const bool few = m <= ddl_few_rows() && n < ((int64_t)1 << 26);  // its grid
+  if (few) {
+    x = inner_contiguous(x);
+    w = inner_contiguous(w);
+  } else {
+    pack(&x, &w);
+  }
+  p.a = x.const_data_ptr();
+  p.lda = row_stride(x);
+  p.b = w.const_data_ptr();
+  p.ldb = row_stride(w);
+  if (few)
+    ddl_product_few(&p, stream_now());
+  else
+    product(p, x);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return y;
 }
 
-// The gradients of linear_fwd that are asked for.  z: what the activation
-// took (its output does for ReLU); not looked at without an activation.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_bwd(
-    at::Tensor dy, at::Tensor x, at::Tensor w, Maybe z, int64_t act,
-    bool want_dx, bool want_dw, bool want_db) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2,
-              "x and weight are matrices on a GPU");
-  TORCH_CHECK(act >= 0 && act <= 4, "unknown activation ", act);
-  const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
-  const int dtype = code_of(x.scalar_type());
-  check_like(w, x, "weight");
-  check_like(dy, x, "dy");
-  check_matrix(w, n, k, "weight");
-  check_matrix(dy, m, n, "dy");
+struct Grads {
+  at::Tensor dx, dw, db;
+};
+
+// z: what the activation took, in float32 (its output, in x's dtype, does for
+// ReLU); not looked at without an activation.  x and w may be padded copies of
+// matrices with k columns.
+Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
+                  const at::Tensor& z, int64_t k, int64_t act, bool want_dx,
+                  bool want_dw, bool want_db) {
   c10::DeviceGuard guard(x.device());
   const auto s = stream_now();
-  at::Tensor dx, dw, db, zc;
-  if (want_dx) dx = at::empty({m, k}, x.options());
-  if (want_dw) dw = at::empty({n, k}, x.options());
-  if (want_db) db = at::empty({n}, x.options());
+  const int64_t m = x.size(0), n = w.size(0);
+  const int dtype = code_of(x.scalar_type());
+  Grads out;
+  if (want_dx) out.dx = at::empty({m, k}, x.options());
+  if (want_dw) out.dw = at::empty({n, k}, x.options());
+  if (want_db) out.db = at::empty({n}, x.options());
   if (m == 0 || n == 0 || k == 0) {  // sums over nothing
-    for (auto* t : {&dx, &dw})
+    for (auto* t : {&out.dx, &out.dw})
       if (t->defined()) t->zero_();
-    if (want_db && m == 0) db.zero_();
+    if (want_db && m == 0) out.db.zero_();
   }
-  if (m == 0 || n == 0) return {dx, dw, db};
+  if (m == 0 || n == 0) return out;
 
-  const at::Tensor d = inner_contiguous(dy);
-  if (act) {
-    TORCH_CHECK(z.has_value(), "the activation's input is missing");
-    check_like(*z, x, "z");
-    check_matrix(*z, m, n, "z");
-    zc = inner_contiguous(*z);
-  }
-  Operand dz{};
+  at::Tensor d = inner_contiguous(dy), dz, zc;
   const bool products = k > 0 && (want_dx || want_dw);
-  if (act && products) {
-    const int64_t wide = round_up(n, 16 / x.element_size());
-    dz.keep = at::empty({m, wide}, x.options());
-    dz.data = dz.keep.const_data_ptr();
-    dz.ld = wide;
+  if (act) {
+    zc = inner_contiguous(z);
+    if (products) dz = at::empty({m, round_up(n, 8)}, x.options());
   }
-  if (want_db || dz.keep.defined()) {
+  if (want_db || dz.defined()) {
     at::Tensor partials;
     if (want_db)
       partials = at::empty({ddl_act_bwd_ws_floats(m, n)},
                            x.options().dtype(at::kFloat));
     ddl_act_bwd(d.const_data_ptr(), row_stride(d),
-                act ? zc.const_data_ptr() : nullptr, act ? row_stride(zc) : 0,
-                dz.keep.defined() ? dz.keep.data_ptr() : nullptr, dz.ld, m, n,
-                (int)act, dtype,
+                act ? zc.const_data_ptr() : nullptr,
+                act && zc.scalar_type() == at::kFloat,
+                act ? row_stride(zc) : 0,
+                dz.defined() ? dz.data_ptr() : nullptr,
+                dz.defined() ? dz.size(1) : 0, m, n, (int)act, dtype,
                 want_db ? partials.data_ptr<float>() : nullptr,
-                want_db ? db.data_ptr() : nullptr, s);
-    C10_HIP_KERNEL_LAUNCH_CHECK();
+                want_db ? out.db.data_ptr() : nullptr, s);
   }
-  if (!products) return {dx, dw, db};
-  if (!act) dz = operand(d);
+  if (products) {
+    if (!act) {
+      dz = d;
+      pack(&dz, want_dx ? &w : nullptr);
+      if (want_dw) pack(&x, nullptr);
+    } else {
+      pack(want_dx ? &w : nullptr, want_dw ? &x : nullptr);
+    }
+    DdlProduct p{};
+    p.dtype = dtype;
+    p.a = dz.const_data_ptr();
+    p.lda = row_stride(dz);
+    p.b_col = 1;
+    p.n = k;
+    p.ldo = k;
+    if (want_dx) {
+      p.b = w.const_data_ptr();
+      p.ldb = row_stride(w);
+      p.m = m;
+      p.r = n;
+      p.out = out.dx.data_ptr();
+      product(p, x);
+    }
+    if (want_dw) {
+      p.b = x.const_data_ptr();
+      p.ldb = row_stride(x);
+      p.a_col = 1;
+      p.m = n;
+      p.r = m;
+      p.out = out.dw.data_ptr();
+      product(p, x);
+    }
+  }
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return out;
+}
 
-  DdlProduct p{};
-  p.dtype = dtype;
-  p.a = dz.data;
-  p.lda = dz.ld;
-  p.b_col = 1;
-  p.n = k;
-  p.ldo = k;
-  if (want_dx) {
-    const Operand b = operand(w);
-    p.b = b.data;
-    p.ldb = b.ld;
-    p.m = m;
-    p.r = n;
-    p.out = dx.data_ptr();
-    product(p, x);
+// Gradients that raise when they are differentiated again.
+variable_list differentiable_once(variable_list grads) {
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "linear_act is differentiable once", (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+class LinearAct : public torch::autograd::Function<LinearAct> {
+ public:
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w,
+                            const Maybe& bias, const Maybe& residual,
+                            int64_t act, bool wants_products) {
+    // ReLU's output tells where its input was positive; with a residual on
+    // top, and for the smooth activations, the input itself is kept
+    const bool by_output = act == 1 && !residual.has_value();
+    const bool want_z = act != 0 && !by_output && wants_products;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["k"] = x.size(1);
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    at::Tensor z;
+    at::Tensor y = forward_of(x, w, bias, residual, act, want_z ? &z : nullptr);
+    ctx->save_for_backward({x, w, by_output ? y : z});
+    return y;
   }
-  if (want_dw) {
-    const Operand b = operand(x);
-    p.b = b.data;
-    p.ldb = b.ld;
-    p.a_col = 1;
-    p.m = n;
-    p.r = m;
-    p.out = dw.data_ptr();
-    product(p, x);
+
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor& dy = dys[0];
+    variable_list out(6);
+    if (!dy.defined()) return out;
+    const bool want_x = ctx->needs_input_grad(0);
+    const bool want_w = ctx->needs_input_grad(1);
+    // tensors that are not there are not counted
+    const bool bias = ctx->saved_data["bias"].toBool();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const bool want_b = bias && ctx->needs_input_grad(2);
+    const bool want_r = residual && ctx->needs_input_grad(bias ? 3 : 2);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (want_x || want_w || want_b) {
+        Grads g = backward_of(dy, saved[0], saved[1], saved[2],
+                              ctx->saved_data["k"].toInt(),
+                              ctx->saved_data["act"].toInt(), want_x, want_w,
+                              want_b);
+        out[0] = g.dx;
+        out[1] = g.dw;
+        out[2] = g.db;
+      }
+    }
+    if (want_r) out[3] = dy;
+    return c10::GradMode::is_enabled() ? differentiable_once(std::move(out))
+                                       : out;
   }
-  return {dx, dw, db};
+};
+
+// functional.linear_act on a GPU.
+at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
+                      const Maybe& bias, int64_t act, Maybe residual) {
+  TORCH_CHECK(x.is_cuda(), "x is on a GPU");
+  TORCH_CHECK_VALUE(act >= 0 && act <= 4, "unknown activation ", act);
+  TORCH_CHECK_VALUE(w.dim() == 2, "weight has shape (out, in), not ",
+                    w.sizes());
+  const int64_t n = w.size(0), k = w.size(1);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "x ends in ", k,
+                    " features, its shape is ", x.sizes());
+  code_of(x.scalar_type());
+  auto like = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type() &&
+                         t.device() == x.device(),
+                     name, " is ", t.scalar_type(), " on ", t.device(),
+                     ", x is ", x.scalar_type(), " on ", x.device());
+  };
+  like(w, "weight");
+  if (bias.has_value()) {
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == n,
+                      "bias has shape (", n, "), not ", bias->sizes());
+    like(*bias, "bias");
+  }
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  if (residual.has_value()) {
+    like(*residual, "residual");
+    bool ok = residual->dim() <= (int64_t)shape.size();
+    for (int64_t d = 1; ok && d <= residual->dim(); ++d)
+      ok = residual->size(-d) == 1 ||
+           residual->size(-d) == shape[shape.size() - d];
+    TORCH_CHECK_VALUE(ok, "residual of shape ", residual->sizes(),
+                      " does not broadcast to ", at::IntArrayRef(shape));
+    if (residual->sizes() != at::IntArrayRef(shape))
+      residual = residual->expand(shape);
+  }
+  const bool matrix = x.dim() == 2;
+  int64_t rows = 1;
+  for (size_t d = 0; d + 1 < shape.size(); ++d) rows *= shape[d];
+  at::Tensor x2 = matrix ? x : x.reshape({rows, k});
+  if (!matrix && residual.has_value()) residual = residual->reshape({rows, n});
+  const bool products =
+      x2.requires_grad() || w.requires_grad() ||
+      (bias.has_value() && bias->requires_grad());
+  const bool any =
+      products || (residual.has_value() && residual->requires_grad());
+  at::Tensor y;
+  if (any && c10::GradMode::is_enabled()) {
+    y = LinearAct::apply(x2, w, bias, residual, act, products);
+  } else {
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor w2 = w;
+    y = forward_of(x2, w2, bias, residual, act, nullptr);
+  }
+  return matrix ? y : y.view(shape);
 }
 
 }  // namespace
 
 void bind_linear(pybind11::module& m) {
-  m.def("linear_fwd", &linear_fwd);
-  m.def("linear_bwd", &linear_bwd);
+  m.def("linear_act", &linear_act);
 }

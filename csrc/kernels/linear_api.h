@@ -24,7 +24,7 @@ struct DdlProduct {
   const void* bias;
   const void* residual;
   int64_t ldres;
-  void* z;              // [m][ldo], z rounded, or null
+  float* z;             // [m][ldo], or null
   int act;
   int dtype;
   float* slabs;         // ddl_product_ws_floats floats
@@ -33,17 +33,29 @@ struct DdlProduct {
 int64_t ddl_product_ws_floats(const DdlProduct* p);
 void ddl_product(const DdlProduct* p, hipStream_t s);
 
-// dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz, and the column
-// sums of the rounded dz: partial sums (ddl_act_bwd_ws_floats floats), then
-// their fold into dbias.  act 1 may take y in the place of z.  dz or dbias
-// may be null.
-int64_t ddl_act_bwd_ws_floats(int64_t m, int64_t n);
-void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz,
-                 void* dz, int64_t lddz, int64_t m, int64_t n, int act,
-                 int dtype, float* partials, void* dbias, hipStream_t s);
+// The same for at most ddl_few_rows() rows, both operands with r contiguous
+// and rows anywhere (any lda, ldb, r and alignment); needs no slabs.
+int ddl_few_rows(void);
+void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
-// dst[i][0..ldd) = src[i][0..n), then zeros.
-void ddl_pack_rows(const void* src, int64_t lds, void* dst, int64_t ldd,
-                   int64_t m, int64_t n, int dtype, hipStream_t s);
+// dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz, and the column
+// sums of dz before its rounding: partial sums (ddl_act_bwd_ws_floats floats),
+// then their fold into dbias.  z is float32 (z_f32), or for act 1 the output
+// in the tensors' dtype.  dz or dbias may be null.
+int64_t ddl_act_bwd_ws_floats(int64_t m, int64_t n);
+void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
+                 int64_t ldz, void* dz, int64_t lddz, int64_t m, int64_t n,
+                 int act, int dtype, float* partials, void* dbias,
+                 hipStream_t s);
+
+// dst[i][0..ldd) = src[i][0..n), then zeros, for one or two matrices; ldd is a
+// multiple of 8, dst of 16 bytes.
+struct DdlPack {
+  const void* src;
+  void* dst;
+  int64_t lds, ldd, m, n;
+};
+void ddl_pack_rows(const DdlPack* matrices, int count, int dtype,
+                   hipStream_t s);
 
 }  // extern "C"

@@ -1,0 +1,7 @@
+// The tiled products of linear_tile.h for one type (a file each, so that they
+// are compiled side by side).
+#include "linear_tile.h"
+
+void ddl_product_f32(const DdlProduct* p, hipStream_t s) {
+  run_product<float>(p, s);
+}

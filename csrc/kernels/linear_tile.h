@@ -1,0 +1,647 @@
+// Products of the dense layer, out = act(x W^T + bias) + residual, and of its
+// backward pass, on matrix instructions.
+//
+// All three products are out[i][j] = sum_r a(i, r) b(j, r):
+//   forward  i = row,     j = output, r = input:  x and W contiguous in r
+//   dx       i = row,     j = input,  r = output: dz in r, W in j
+//   dW       i = output,  j = input,  r = row:    dz in i, x in j
+// so an operand lies with r contiguous ("row") or with its output index
+// contiguous ("col"), and nothing is transposed in memory.
+//
+// Tiles go from memory to LDS by buffer loads (16 B a lane, no registers in
+// between) into a ring of stages.  Reads past an operand's end return zeros by the
+// buffer's own bounds check; r's ragged end is cut by moving a lane's offset
+// out of bounds.
+//
+// LDS images (16-byte units, one 128-byte line of a row operand or one line
+// of a col operand after the other).  A wave's loads fill LDS in lane order,
+// so units are exchanged on the source side: unit u of line l is stored at
+// place u ^ f(l), with f chosen such that the 16 lanes of a fragment read
+// touch all banks.  Fragments of 2-byte col operands come out of
+// ds_read_b64_tr_b16, which transposes 4 x 16 elements among 16 lanes.
+//
+// The b fragment is the first operand of the matrix instruction and its rows
+// are dealt so that a lane ends up with 16 consecutive j of one row i.
+//
+// Compiled without fast-math: infinities and NaN keep their meaning.
+#pragma once
+#include "common.h"
+#include "linear_api.h"
+
+#include <type_traits>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) unsigned int lds_u32;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+constexpr int LINE = 128;            // bytes of r a step takes of a row
+constexpr uint32_t OUTSIDE = 0x80000000u;  // past every buffer's end
+
+struct Epilogue {
+  const void* bias;
+  const void* residual;
+  void* out;
+  float* z;
+  int64_t ldo, ldres, m, n;
+  int act;
+  int wide;  // rows of out, z and residual take 16-byte accesses
+};
+
+struct Product {
+  const char* a;
+  const char* b;
+  int64_t lda, ldb;  // bytes
+  int64_t r;         // reduction length, padded to 16 bytes for row operands
+  int64_t steps;     // r in steps of LINE bytes
+  int64_t steps_per_split;
+  int splits, tiles_m, tiles_n;
+  float* slabs;
+  int64_t ldslab;
+  Epilogue e;
+};
+
+// ---- activations -----------------------------------------------------------
+
+__device__ __forceinline__ float sigmoid(float z) {
+  return 1.f / (1.f + __expf(-z));
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case 1: return z < 0.f ? 0.f : z;  // NaN passes
+    case 2: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case 3: {
+      // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+      const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
+      return z * sigmoid(u);
+    }
+    case 4: return z * sigmoid(z);
+    default: return z;
+  }
+}
+
+__device__ __forceinline__ float activate_grad(float z, int act) {
+  switch (act) {
+    case 1: return z <= 0.f ? 0.f : 1.f;
+    case 2:
+      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
+             z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case 3: {
+      const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
+      const float s = sigmoid(u);
+      return s + z * s * (1.f - s) *
+                     (1.5957691216057308f * (1.f + 0.134145f * z * z));
+    }
+    case 4: {
+      const float s = sigmoid(z);
+      return s * (1.f + z * (1.f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+// ---- matrix instructions ---------------------------------------------------
+
+// A fragment is 16 bytes a lane: of row (lane & 15), elements
+// (lane >> 4) * E + 0..E-1 of 4 E consecutive r, E = 16 / sizeof(T).
+template <typename T> struct Frag;
+template <> struct Frag<bf16> { using type = bf16x8; };
+template <> struct Frag<f16> { using type = f16x8; };
+template <> struct Frag<float> { using type = f32x4; };
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// ---- epilogue --------------------------------------------------------------
+
+// `fn` on 8 values; the switch stands outside, so that the code of one
+// activation is run through without a branch an element.
+__device__ __forceinline__ void activate8(float* y, int act) {
+  auto all = [&](auto which) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = activate(y[k], which.value);
+  };
+  switch (act) {
+    case 1: all(std::integral_constant<int, 1>{}); break;
+    case 2: all(std::integral_constant<int, 2>{}); break;
+    case 3: all(std::integral_constant<int, 3>{}); break;
+    case 4: all(std::integral_constant<int, 4>{}); break;
+  }
+}
+
+// Columns j..j+7 of row i; `sum` is the product.
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t i,
+                                        int64_t j, const float* sum,
+                                        const float* bias) {
+  float z[8], y[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y[k] = z[k] = sum[k] + bias[k];
+  activate8(y, e.act);
+  T* out = (T*)e.out + i * e.ldo + j;
+  float* zout = e.z ? e.z + i * e.ldo + j : nullptr;
+  const T* res =
+      e.residual ? (const T*)e.residual + i * e.ldres + j : nullptr;
+  if (e.wide && j + 8 <= e.n) {
+    Vec8<T> o;
+    if (res) {
+      const Vec8<T> r = load8(res);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] += to_f32(r.v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(y[k]);
+    store8(out, o);
+    if (zout) {
+      Vec8<float> q;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q.v[k] = z[k];
+      store8(zout, q);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (j + k < e.n) {
+        out[k] = from_f32<T>(res ? y[k] + to_f32(res[k]) : y[k]);
+        if (zout) zout[k] = z[k];
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias8(const Epilogue& e, int64_t j,
+                                           float* bias) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    bias[k] = e.bias && j + k < e.n ? to_f32(((const T*)e.bias)[j + k]) : 0.f;
+}
+
+template <typename T> Epilogue epilogue_of(const DdlProduct* d) {
+  const int64_t per = 16 / (int)sizeof(T);
+  auto wide = [&](const void* p, int64_t ld) {
+    return ((uintptr_t)p & 15) == 0 && ld % per == 0;
+  };
+  return Epilogue{d->bias, d->residual, d->out, d->z, d->ldo, d->ldres, d->m,
+                  d->n, d->act,
+                  wide(d->out, d->ldo) &&
+                      (!d->residual || wide(d->residual, d->ldres))};
+}
+
+// ---- the tiled product -----------------------------------------------------
+
+// Place of unit u of line l is u ^ swizzle(l); UNITS: units of a line.
+template <typename T, bool COL, bool IS_B, int UNITS>
+__device__ __forceinline__ int swizzle(int l) {
+  if constexpr (!COL) {
+    // a reads lines x = 0..15 at one unit, b lines (x >> 2) * 16 + (x & 3)
+    return IS_B ? (l & 3) | (((l >> 4) & 1) << 2) : l & 7;
+  } else if constexpr (sizeof(T) == 2 && UNITS >= 16) {
+    // 4 lines a 16-lane group; a: 2 neighbouring units, b: 4 units, 2 apart
+    return IS_B ? (l & 1) | (((l >> 1) & 1) << 3)
+                : ((l & 3) << 1) | (((l >> 3) & 1) << 3);
+  } else if constexpr (sizeof(T) == 2) {
+    // two lines of 8 units lie side by side over the banks
+    static_assert(UNITS == 8, "a line is 128 bytes or more");
+    return IS_B ? (l >> 1) & 1
+                : (((l >> 1) & 1) << 1) | (((l >> 3) & 1) << 2);
+  } else {
+    static_assert(UNITS >= 16, "a line is 256 bytes or more");
+    return IS_B ? (l >> 2) & 3 : ((l >> 2) & 3) << 2;
+  }
+}
+
+// One operand's tile of W output indexes: ROWS lines in memory and in LDS.
+template <typename T, bool COL, bool IS_B, int W, int WAVES>
+struct Tile {
+  static constexpr int BYTES = W * LINE;
+  static constexpr int LOADS = BYTES / (WAVES * 1024);
+  static constexpr int UNITS = COL ? W * (int)sizeof(T) / 16 : LINE / 16;
+  static constexpr int STEP = LINE / (int)sizeof(T);  // elements of r
+  static_assert(BYTES % (WAVES * 1024) == 0, "whole loads");
+
+  // LDS instructions a fragment
+  static constexpr int READS = !COL ? 1 : sizeof(T) == 2 ? 2 : 4;
+
+  uint32_t offset[LOADS];   // of this lane's 16 bytes from the tile's start
+  uint32_t along[LOADS];    // its place in r: bytes (row) or lines (col)
+
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld,
+                                       int64_t indexes) {
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+      const int u = (q * WAVES + wave) * 64 + lane;
+      const int line = u / UNITS;
+      const int unit = (u % UNITS) ^ swizzle<T, COL, IS_B, UNITS>(line);
+      const int64_t index = COL ? unit * (16 / (int)sizeof(T)) : line;
+      along[q] = COL ? line : unit * 16;
+      offset[q] = index < indexes ? (uint32_t)(line * ld) + unit * 16 : OUTSIDE;
+    }
+  }
+
+  // Loads the tile at `base`; `end`: bytes from there to the operand's end;
+  // `left`: what is left of r, in `along`'s measure (0: zeros are loaded).
+  __device__ __forceinline__ void load(char* __restrict lds, int wave, const char* base,
+                                       int64_t end, uint32_t left) const {
+    const int records = (int)max(min(end, (int64_t)0x7FFFFFFF), (int64_t)0);
+    __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(base), 0, records, 0x00020000);
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+      const uint32_t o = along[q] < left ? offset[q] : OUTSIDE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (lds_u32*)(lds + (q * WAVES + wave) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+
+  // Fragment number f (16 indexes) of the wave's part that starts at index w;
+  // half kk of the step.
+  __device__ __forceinline__ typename Frag<T>::type read(const char* __restrict lds,
+                                                         int lane, int w,
+                                                         int f, int kk) const {
+    const int x = lane & 15, g = lane >> 4;
+    // b's rows: 16 consecutive j of a lane are spread over 4 fragments
+    auto index = [&](int y) {
+      return IS_B ? w + (f >> 2) * 64 + (y >> 2) * 16 + (f & 3) * 4 + (y & 3)
+                  : w + f * 16 + y;
+    };
+    if constexpr (!COL) {
+      const int line = index(x);
+      const int unit = (kk * 4 + g) ^ swizzle<T, COL, IS_B, UNITS>(line);
+      return *reinterpret_cast<const typename Frag<T>::type*>(
+          lds + line * LINE + unit * 16);
+    } else if constexpr (sizeof(T) == 2) {
+      typename Frag<T>::type out;
+      s16x4* half = reinterpret_cast<s16x4*>(&out);
+      const int first = index((x & 3) * 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int line = kk * 32 + g * 8 + h * 4 + (x >> 2);
+        const int unit = (first >> 3) ^ swizzle<T, COL, IS_B, UNITS>(line);
+        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(
+            lds + line * (W * 2) + unit * 16 + (first & 7) * 2));
+      }
+      return out;
+    } else {
+      typename Frag<T>::type out;
+      const int i = index(x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int line = kk * 16 + g * 4 + e;
+        const int unit = (i >> 2) ^ swizzle<T, COL, IS_B, UNITS>(line);
+        out[e] = *reinterpret_cast<const float*>(lds + line * (W * 4) +
+                                                 unit * 16 + (i & 3) * 4);
+      }
+      return out;
+    }
+  }
+};
+
+// Waits until at most LOADS of this wave's loads are under way and its LDS
+// reads have returned, then for the block's other waves to say the same.
+template <int LOADS>
+__device__ __forceinline__ void meet() {
+  static_assert(LOADS < 64, "the counter's range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Lets the scheduler spread LDS reads and loads evenly among the matrix
+// instructions of a block: issued in one go, they fill the LDS queue and hold
+// the matrix instructions back.
+template <int READS, int MATRIX, int LOADS>
+__device__ __forceinline__ void interleave() {
+  constexpr int PAIRS = READS > MATRIX / 2 ? 2 : 1;  // reads a matrix instr.
+#pragma unroll
+  for (int i = 0; i < READS / PAIRS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, PAIRS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, MATRIX - READS / PAIRS, 0);
+}
+
+// The epilogue of a block: each wave lays its sums into its own part of LDS,
+// 64 columns a line, and takes them back 8 columns a lane: whole lines go to
+// memory, and the epilogue's code is there once (unrolled over the registers
+// it was so long that fetching it cost 40 us a tile).  16-byte units are
+// exchanged within a line by its row, which spreads both accesses over the
+// banks.  `smem` holds BYTES that no wave uses any more.
+template <typename T, int MI, int NI, int WAVES, int BYTES>
+__device__ __forceinline__ void write_out(const Product& p, char* smem,
+                                          const f32x4 (&acc)[MI][NI],
+                                          int wave, int lane, int split,
+                                          int64_t i0, int64_t j0) {
+  constexpr int PASS = WAVES * MI * 16 * 256 <= BYTES ? MI : MI / 2;
+  constexpr int ROWS = PASS * 16;
+  static_assert(WAVES * ROWS * 256 <= BYTES, "sums fit the tiles' LDS");
+  float* sums = reinterpret_cast<float*>(smem) + wave * ROWS * 64;
+  const int x = lane & 15, g = lane >> 4;
+  const int row = lane >> 3, unit = (lane & 7) * 2;
+#pragma unroll
+  for (int h = 0; h < NI / 4; ++h) {
+    const int64_t j = j0 + h * 64 + (lane & 7) * 8;
+    float bias[8];
+    if (p.splits == 1) load_bias8<T>(p.e, j, bias);
+#pragma unroll
+    for (int f0 = 0; f0 < MI; f0 += PASS) {
+#pragma unroll
+      for (int f = 0; f < PASS; ++f)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(sums + (f * 16 + x) * 64 +
+                                    ((g * 4 + q) ^ x) * 4) =
+              acc[f0 + f][h * 4 + q];
+      // A wave's LDS accesses are done in order: no barrier within a wave.
+#pragma unroll 1
+      for (int r = row; r < ROWS; r += 8) {
+        const int64_t i = i0 + f0 * 16 + r;
+        union { f32x4 v[2]; float f[8]; } sum;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          sum.v[q] = *reinterpret_cast<const f32x4*>(
+              sums + r * 64 + ((unit + q) ^ (r & 15)) * 4);
+        if (i >= p.e.m || j >= p.e.n) continue;
+        if (p.splits > 1) {
+          // rows of a slab are padded to 8 numbers
+          float* s = p.slabs + (split * p.e.m + i) * p.ldslab + j;
+          *reinterpret_cast<f32x4*>(s) = sum.v[0];
+          *reinterpret_cast<f32x4*>(s + 4) = sum.v[1];
+        } else {
+          finish8<T>(p.e, i, j, sum.f, bias);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_COL,
+          bool B_COL>
+__global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
+  constexpr int WAVES = WM * WN;
+  constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  static_assert(NI % 4 == 0, "a lane's 16 columns are 4 fragments");
+  using TA = Tile<T, A_COL, false, BM, WAVES>;
+  using TB = Tile<T, B_COL, true, BN, WAVES>;
+  constexpr int STAGE = TA::BYTES + TB::BYTES;
+  __shared__ __align__(16) char smem[STAGES * STAGE];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = p.tiles_m * p.tiles_n;
+  const unsigned id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int split = id / tiles;
+  const int tile = id % tiles;
+  // i runs fastest: neighbours on an XCD share the b tile
+  const int64_t i0 = (int64_t)(tile % p.tiles_m) * BM;
+  const int64_t j0 = (int64_t)(tile / p.tiles_m) * BN;
+
+  TA ta;
+  TB tb;
+  ta.init(wave, lane, p.lda, p.e.m - i0);
+  tb.init(wave, lane, p.ldb, p.e.n - j0);
+
+  const int64_t t0 = split * p.steps_per_split;
+  const int64_t t1 = min(p.steps, t0 + p.steps_per_split);
+  constexpr int64_t STEP = TA::STEP;
+  // bytes from a tile's start to the operand's end
+  const char* a = p.a + (A_COL ? i0 * (int64_t)sizeof(T) : i0 * p.lda);
+  const char* b = p.b + (B_COL ? j0 * (int64_t)sizeof(T) : j0 * p.ldb);
+  const int64_t a_all = A_COL
+      ? (p.r - 1) * p.lda + (p.e.m - i0) * (int64_t)sizeof(T)
+      : (p.e.m - i0 - 1) * p.lda + p.r * (int64_t)sizeof(T);
+  const int64_t b_all = B_COL
+      ? (p.r - 1) * p.ldb + (p.e.n - j0) * (int64_t)sizeof(T)
+      : (p.e.n - j0 - 1) * p.ldb + p.r * (int64_t)sizeof(T);
+  // what is contiguous is a multiple of 16 bytes long
+  const int64_t a_end = (a_all + 15) & ~(int64_t)15;
+  const int64_t b_end = (b_all + 15) & ~(int64_t)15;
+
+  auto load = [&](int64_t t, int stage) {
+    char* l = smem + stage * STAGE;
+    const int64_t ao = A_COL ? t * STEP * p.lda : t * LINE;
+    const int64_t bo = B_COL ? t * STEP * p.ldb : t * LINE;
+    // past this block's part of r nothing is read
+    const int64_t left =
+        t < t1 ? min(p.r - t * STEP, (int64_t)STEP) : (int64_t)0;
+    const uint32_t lines = (uint32_t)left;
+    const uint32_t bytes = (uint32_t)(left * (int)sizeof(T));
+    ta.load(l, wave, a + ao, a_end - ao, A_COL ? lines : bytes);
+    tb.load(l + TA::BYTES, wave, b + bo, b_end - bo, B_COL ? lines : bytes);
+  };
+
+  f32x4 acc[MI][NI] = {};
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+
+  // Half a step's fragments are read while the other half's products run.
+  // Once a step, in its middle: the next tile has landed and this wave's reads
+  // of the present one have returned; past the barrier both hold for all
+  // waves, so the present stage is loaded anew, STAGES - 1 steps ahead.  Loads
+  // past the end are issued too, and read nothing: their number is the same
+  // in every step.
+  using F = typename Frag<T>::type;
+  F a0[MI], b0[NI], a1[MI], b1[NI];
+  auto read = [&](F (&af)[MI], F (&bf)[NI], int stage, int kk) {
+    const char* la = smem + stage * STAGE;
+#pragma unroll
+    for (int f = 0; f < NI; ++f)
+      bf[f] = tb.read(la + TA::BYTES, lane, wn, f, kk);
+#pragma unroll
+    for (int f = 0; f < MI; ++f) af[f] = ta.read(la, lane, wm, f, kk);
+  };
+  auto multiply = [&](const F (&af)[MI], const F (&bf)[NI]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = mma(bf[j], af[i], acc[i][j]);
+  };
+  constexpr int PER = sizeof(T) == 4 ? 4 : 1;  // instructions a fragment pair
+  constexpr int READS = MI * TA::READS + NI * TB::READS;
+  constexpr int LOADS = TA::LOADS + TB::LOADS;
+  if (t0 < t1) {
+#pragma unroll
+    for (int q = 0; q < STAGES; ++q) load(t0 + q, q);
+    meet<(STAGES - 1) * LOADS>();
+    read(a0, b0, 0, 0);
+    int stage = 0;
+    for (int64_t t = t0; t + 1 < t1; ++t) {
+      const int next = stage + 1 < STAGES ? stage + 1 : 0;
+      read(a1, b1, stage, 1);
+      multiply(a0, b0);
+      interleave<READS, MI * NI * PER, 0>();
+      meet<(STAGES - 2) * LOADS>();
+      load(t + STAGES, stage);
+      read(a0, b0, next, 0);
+      multiply(a1, b1);
+      interleave<READS, MI * NI * PER, LOADS>();
+      stage = next;
+    }
+    read(a1, b1, stage, 1);
+    multiply(a0, b0);
+    multiply(a1, b1);
+  }
+
+  meet<0>();
+  write_out<T, MI, NI, WAVES, STAGES * STAGE>(p, smem, acc, wave, lane, split,
+                                              i0 + wm, j0 + wn);
+}
+
+// Adds the slabs in order (no atomics: the result does not depend on which
+// block ends first) and applies the epilogue; 8 columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void join_k(const float* slabs, int splits,
+                                              int64_t ldslab, Epilogue e) {
+  const int64_t groups = ldslab / 8;
+  const int64_t at = global_tid();
+  if (at >= groups * e.m) return;
+  const int64_t i = at / groups, j = (at % groups) * 8;
+  if (j >= e.n) return;
+  float sum[8] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float* q = slabs + (s * e.m + i) * ldslab + j;
+    const float4 lo = *reinterpret_cast<const float4*>(q);
+    const float4 hi = *reinterpret_cast<const float4*>(q + 4);
+    sum[0] += lo.x; sum[1] += lo.y; sum[2] += lo.z; sum[3] += lo.w;
+    sum[4] += hi.x; sum[5] += hi.y; sum[6] += hi.z; sum[7] += hi.w;
+  }
+  float bias[8];
+  load_bias8<T>(e, j, bias);
+  finish8<T>(e, i, j, sum, bias);
+}
+
+// ---- host ------------------------------------------------------------------
+
+inline int compute_units() {
+  static const int n = [] {
+    hipDeviceProp_t prop;
+    return hipGetDeviceProperties(&prop, 0) == hipSuccess
+               ? prop.multiProcessorCount : 256;
+  }();
+  return n;
+}
+
+inline bool takes16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Tile sizes, blocks a compute unit holds, and measured times in us: of a
+// step (128 bytes of r) where a unit holds one block and where it is full,
+// and of a block's beginning and end.
+struct TileKind {
+  int side, per_unit;
+  float alone, full, ends;
+};
+
+// bf16 and f16.  4096^3, forward / dx / dW: 256 takes 104 / 103 / 107 us, 128
+// 122 / 134 / 152, 64 307 / 300 / 301; 256 x 2048 x 1000 split for each: 64
+// takes 11 / 10 / 7, 128 13 / 14 / 9, 256 16 and more.
+constexpr TileKind KINDS16[] = {{256, 1, 1.2f, 1.5f, 7.f},
+                                {128, 2, 0.68f, 0.95f, 3.f},
+                                {64, 2, 0.23f, 0.6f, 1.5f}};
+// float32: 4096^3 980 (128) against 1127 (64); 256 x 2048 x 1000 19 (64)
+// against 26.
+constexpr TileKind KINDS32[] = {{128, 2, 2.0f, 3.8f, 3.f},
+                                {64, 2, 0.6f, 1.1f, 1.5f}};
+
+struct Plan {
+  TileKind kind;
+  int splits;
+  int64_t steps, steps_per_split;
+};
+
+// The tile and the split of r with the smallest estimate: rounds of blocks
+// over the compute units, and for a split the launch that joins its slabs
+// (4 us and their bytes, written and read, at 10 TB/s: they stay in the last
+// level cache).
+inline Plan plan_of(const DdlProduct* p) {
+  const int size = p->dtype == 0 ? 4 : 2;
+  const int64_t steps = cdiv(p->r * size, LINE);
+  Plan best{};
+  float best_us = 0.f;
+  auto consider = [&](const TileKind& k) {
+    const int64_t tiles = cdiv(p->m, k.side) * cdiv(p->n, k.side);
+    for (int64_t s = 1; s <= 32; ++s) {
+      if (s > 1 && steps < 2 * s) break;
+      const int64_t per = std::max<int64_t>(1, cdiv(steps, s));
+      const int64_t splits = std::max<int64_t>(1, cdiv(steps, per));
+      if (splits != s) continue;
+      const int64_t blocks = tiles * splits;
+      const int64_t rounds =
+          cdiv(blocks, (int64_t)compute_units() * k.per_unit);
+      const float step = blocks <= compute_units() ? k.alone : k.full;
+      float us = rounds * (k.ends + per * step);
+      if (splits > 1) us += 4.f + splits * p->m * p->n * 8e-7f;
+      if (best.kind.side == 0 || us < best_us) {
+        best_us = us;
+        best = Plan{k, (int)splits, steps, per};
+      }
+    }
+  };
+  if (p->dtype == 0)
+    for (const auto& k : KINDS32) consider(k);
+  else
+    for (const auto& k : KINDS16) consider(k);
+  return best;
+}
+
+template <typename T, int SIDE, int WM, int WN, int STAGES>
+void launch_product(const Product& p, int a_col, int b_col, hipStream_t s) {
+  const dim3 grid(p.tiles_m * p.tiles_n * p.splits), block(WM * WN * 64);
+  if (a_col && b_col)
+    product_k<T, SIDE, SIDE, WM, WN, STAGES, true, true>
+        <<<grid, block, 0, s>>>(p);
+  else if (b_col)
+    product_k<T, SIDE, SIDE, WM, WN, STAGES, false, true>
+        <<<grid, block, 0, s>>>(p);
+  else
+    product_k<T, SIDE, SIDE, WM, WN, STAGES, false, false>
+        <<<grid, block, 0, s>>>(p);
+}
+
+template <typename T>
+void run_product(const DdlProduct* d, hipStream_t s) {
+  const Plan plan = plan_of(d);
+  Product p{};
+  p.a = (const char*)d->a;
+  p.b = (const char*)d->b;
+  p.lda = d->lda * (int64_t)sizeof(T);
+  p.ldb = d->ldb * (int64_t)sizeof(T);
+  p.r = d->r;
+  p.steps = plan.steps;
+  p.steps_per_split = plan.steps_per_split;
+  p.splits = plan.splits;
+  p.tiles_m = (int)cdiv(d->m, plan.kind.side);
+  p.tiles_n = (int)cdiv(d->n, plan.kind.side);
+  p.slabs = d->slabs;
+  p.ldslab = cdiv(d->n, 8) * 8;
+  p.e = epilogue_of<T>(d);
+  if (plan.kind.side == 256) {
+    if constexpr (sizeof(T) == 2)
+      launch_product<T, 256, 2, 4, 2>(p, d->a_col, d->b_col, s);
+  } else if (plan.kind.side == 128) {
+    launch_product<T, 128, 2, 2, 2>(p, d->a_col, d->b_col, s);
+  } else {
+    launch_product<T, 64, 4, 1, 4>(p, d->a_col, d->b_col, s);
+  }
+  if (p.splits > 1) {
+    const int64_t threads = p.ldslab / 8 * d->m;
+    join_k<T><<<(unsigned)cdiv(threads, 256), 256, 0, s>>>(
+        p.slabs, p.splits, p.ldslab, p.e);
+  }
+}
+
+}  // namespace

@@ -16,12 +16,10 @@ from __future__ import annotations
 
 from typing import Optional
 
-import math
 import os
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from ._ext import load_kernels_ext
 
@@ -442,33 +440,6 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _DENSE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-class _LinearActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        ext = load_kernels_ext()
-        # ReLU's output tells where its input was positive; with a residual
-        # on top, and for the smooth activations, the input itself is kept
-        by_output = act == ACTIVATIONS["relu"] and residual is None
-        want_z = act != 0 and not by_output and any(ctx.needs_input_grad[:3])
-        y, z = ext.linear_fwd(x, weight, bias, residual, act, want_z)
-        ctx.act = act
-        kept = y if by_output else z if want_z else None
-        ctx.save_for_backward(x, weight, kept)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        ext = load_kernels_ext()
-        x, weight, kept = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            dx, dw, db = ext.linear_bwd(dy, x, weight, kept, ctx.act, need_x,
-                                        need_w, need_b)
-        return dx, dw, db, dy if need_r else None, None
-
-
 def _cpu_activation(z, activation):
     if activation == "relu":
         return F.relu(z)
@@ -494,6 +465,9 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, not "
                          f"{activation!r}")
+    if x.is_cuda:
+        return load_kernels_ext().linear_act(
+            x, weight, bias, ACTIVATIONS[activation], residual)
     if weight.dim() != 2:
         raise ValueError(f"weight has shape (out, in), not {tuple(weight.shape)}")
     out, inp = weight.shape
@@ -516,19 +490,12 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         except RuntimeError as e:
             raise ValueError(f"residual of shape {tuple(residual.shape)} does "
                              f"not broadcast to {tuple(shape)}") from e
-    if not x.is_cuda:
-        z = F.linear(x.float(), weight.float(),
-                     None if bias is None else bias.float())
-        y = _cpu_activation(z, activation)
-        if residual is not None:
-            y = y + residual.float()
-        return y.to(x.dtype)
-    rows = math.prod(shape[:-1])
-    y = _LinearActFn.apply(
-        x.reshape(rows, inp), weight, bias,
-        None if residual is None else residual.reshape(rows, out),
-        ACTIVATIONS[activation])
-    return y.view(shape)
+    z = F.linear(x.float(), weight.float(),
+                 None if bias is None else bias.float())
+    y = _cpu_activation(z, activation)
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)
 
 
 # --------------------------------------------------------------------------

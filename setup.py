@@ -38,7 +38,8 @@ HIPCC_FLAGS = [
 ]
 # Kernels that keep IEEE meaning (infinities and NaN in inputs, correctly
 # rounded division and roots) are compiled without fast-math.
-IEEE_KERNELS = {"adamw", "linear"}
+IEEE_KERNELS = {"adamw", "linear", "linear_bf16", "linear_f16",
+                "linear_f32"}
 
 
 def compile_hip_objects() -> list:
