@@ -78,11 +78,10 @@ void pack(at::Tensor* a, at::Tensor* b) {
   if (count) ddl_pack_rows(todo, count, dtype, stream_now());
 }
 
-// out = epilogue(a b^T) with its workspace.
-void product(DdlProduct& p, const at::Tensor& like) {
-  if (p.m == 0 || p.n == 0) return;
+// out = epilogue(a b^T) with its workspace; `p` is planned, and holds something.
+void product(DdlProduct& p, int64_t floats, const at::Tensor& like) {
   at::Tensor slabs;
-  if (const int64_t floats = ddl_product_ws_floats(&p)) {
+  if (floats) {
     slabs = at::empty({floats}, like.options().dtype(at::kFloat));
     p.slabs = slabs.data_ptr<float>();
   }
@@ -135,7 +134,7 @@ at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
   if (few)
     ddl_product_few(&p, stream_now());
   else
-    product(p, x);
+    product(p, ddl_product_plan(&p), x);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return y;
 }
@@ -171,20 +170,24 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
     zc = inner_contiguous(z);
     if (products) dz = at::empty({m, round_up(n, 8)}, x.options());
   }
-  if (want_db || dz.defined()) {
-    at::Tensor partials;
-    if (want_db)
-      partials = at::empty({ddl_act_bwd_ws_floats(m, n)},
-                           x.options().dtype(at::kFloat));
+  DdlBiasFold fold{};
+  at::Tensor partials;
+  if (want_db) {
+    fold.chunks = ddl_bias_chunks(m);
+    fold.n = n;
+    partials = at::empty({fold.chunks * n}, x.options().dtype(at::kFloat));
+    fold.partials = partials.data_ptr<float>();
+    fold.dbias = out.db.data_ptr();
+  }
+  if (want_db || dz.defined())
     ddl_act_bwd(d.const_data_ptr(), row_stride(d),
                 act ? zc.const_data_ptr() : nullptr,
                 act && zc.scalar_type() == at::kFloat,
                 act ? row_stride(zc) : 0,
                 dz.defined() ? dz.data_ptr() : nullptr,
                 dz.defined() ? dz.size(1) : 0, m, n, (int)act, dtype,
-                want_db ? partials.data_ptr<float>() : nullptr,
-                want_db ? out.db.data_ptr() : nullptr, s);
-  }
+                want_db ? partials.data_ptr<float>() : nullptr, s);
+  DdlProduct px{}, pw{};
   if (products) {
     if (!act) {
       dz = d;
@@ -193,31 +196,35 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
     } else {
       pack(want_dx ? &w : nullptr, want_dw ? &x : nullptr);
     }
-    DdlProduct p{};
-    p.dtype = dtype;
-    p.a = dz.const_data_ptr();
-    p.lda = row_stride(dz);
-    p.b_col = 1;
-    p.n = k;
-    p.ldo = k;
-    if (want_dx) {
-      p.b = w.const_data_ptr();
-      p.ldb = row_stride(w);
-      p.m = m;
-      p.r = n;
-      p.out = out.dx.data_ptr();
-      product(p, x);
-    }
-    if (want_dw) {
-      p.b = x.const_data_ptr();
-      p.ldb = row_stride(x);
-      p.a_col = 1;
-      p.m = n;
-      p.r = m;
-      p.out = out.dw.data_ptr();
-      product(p, x);
+    px.dtype = dtype;
+    px.a = dz.const_data_ptr();
+    px.lda = row_stride(dz);
+    px.b_col = 1;
+    px.n = k;
+    px.ldo = k;
+    pw = px;
+    px.b = w.const_data_ptr();
+    px.ldb = row_stride(w);
+    px.m = m;
+    px.r = n;
+    pw.b = x.const_data_ptr();
+    pw.ldb = row_stride(x);
+    pw.a_col = 1;
+    pw.m = n;
+    pw.r = m;
+    if (want_dx) px.out = out.dx.data_ptr();
+    if (want_dw) pw.out = out.dw.data_ptr();
+    const int64_t fx = want_dx ? ddl_product_plan(&px) : 0;
+    const int64_t fw = want_dw ? ddl_product_plan(&pw) : 0;
+    if (want_dx && want_dw && ddl_small_backward(&px, &pw)) {
+      ddl_backward_small(&px, &pw, &fold, s);
+      fold.n = 0;
+    } else {
+      if (want_dx) product(px, fx, x);
+      if (want_dw) product(pw, fw, x);
     }
   }
+  if (fold.n) ddl_fold_bias(&fold, dtype, s);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return out;
 }

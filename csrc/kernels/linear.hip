@@ -3,9 +3,15 @@
 // in linear_tile.h.
 #include "linear_tile.h"
 
-void ddl_product_bf16(const DdlProduct* p, hipStream_t s);
-void ddl_product_f16(const DdlProduct* p, hipStream_t s);
-void ddl_product_f32(const DdlProduct* p, hipStream_t s);
+#define DDL_TYPE(NAME)                                                    \
+  void ddl_product_##NAME(const DdlProduct* p, hipStream_t s);            \
+  void ddl_backward_small_##NAME(const DdlProduct* dx,                    \
+                                 const DdlProduct* dw,                    \
+                                 const DdlBiasFold* bias, hipStream_t s);
+DDL_TYPE(f32)
+DDL_TYPE(bf16)
+DDL_TYPE(f16)
+#undef DDL_TYPE
 
 namespace {
 
@@ -111,7 +117,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
 template <typename T, int MT>
 void launch_few(const DdlProduct* p, hipStream_t s) {
   few_rows_k<T, MT, 16><<<(unsigned)cdiv(p->n, 16), 1024, 0, s>>>(
-      (const T*)p->a, p->lda, (const T*)p->b, p->ldb, p->r, epilogue_of<T>(p));
+      (const T*)p->a, p->lda, (const T*)p->b, p->ldb, p->r, epilogue_of(p));
 }
 
 template <typename T>
@@ -125,57 +131,57 @@ void run_few(const DdlProduct* p, hipStream_t s) {
 constexpr int BWD_ROWS = 32;   // rows a block sums
 constexpr int BWD_COLS = 256;  // 32 threads of 8 columns
 
-// Elements j..j+7 of a row of n, zeros behind its end.
+// Elements j..j+7 of a row of n, zeros behind its end; it may begin anywhere.
 template <typename T>
-__device__ __forceinline__ Vec8<T> row8(const T* row, int64_t j, int64_t n,
-                                        bool wide) {
-  if (wide && j + 8 <= n) return load8(row + j);
-  Vec8<T> r;
+__device__ __forceinline__ void row8(const T* row, int64_t j, int64_t n,
+                                     float* out) {
+  T r[8];
+  if (j + 8 <= n) {
+    __builtin_memcpy(r, row + j, sizeof(r));
+  } else {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    r.v[k] = j + k < n ? row[j + k] : from_f32<T>(0.f);
-  return r;
+    for (int k = 0; k < 8; ++k)
+      r[k] = j + k < n ? row[j + k] : from_f32<T>(0.f);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) out[k] = to_f32(r[k]);
 }
 
 template <typename T, typename Z>
 __global__ __launch_bounds__(256) void act_bwd_k(
     const T* __restrict__ dy, int64_t lddy, const Z* __restrict__ z,
     int64_t ldz, T* __restrict__ dz, int64_t lddz, int64_t m, int64_t n,
-    int act, int wide, float* __restrict__ partials) {
+    int act, float* __restrict__ partials) {
   __shared__ float part[8][BWD_COLS];
   const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
   const int64_t col_blocks = cdiv(n, BWD_COLS);
   const int64_t cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks;
   const int64_t j = cb * BWD_COLS + cg * 8;
-  float sum[8] = {};
-  for (int64_t i = rb * BWD_ROWS + rg;
-       i < min(m, (rb + 1) * (int64_t)BWD_ROWS) && j < n; i += 8) {
-    const Vec8<T> d = row8(dy + i * lddy, j, n, wide & 1);
-    float v[8];
+  constexpr int TURNS = BWD_ROWS / 8;
+  float v[TURNS][8], q[TURNS][8], sum[8] = {};
+  const int64_t i0 = rb * BWD_ROWS + rg;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = to_f32(d.v[k]);
-    if (act) {
-      const Vec8<Z> q = row8(z + i * ldz, j, n, wide & 2);
+  for (int t = 0; t < TURNS; ++t) {  // all loads first
+    const int64_t i = i0 + t * 8;
+    const int64_t end = i < m ? n : 0;  // rows past the end are empty
+    row8(dy + (i < m ? i * lddy : 0), j, end, v[t]);
+    if (act) row8(z + (i < m ? i * ldz : 0), j, end, q[t]);
+  }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= activate_grad(to_f32(q.v[k]), act);
-    }
+  for (int t = 0; t < TURNS; ++t) {
+    if (act) activate_grad8(v[t], q[t], act);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (j + k >= n) v[k] = 0.f;
-      sum[k] += v[k];
+      // a gradient of NaN behind the row's end would enter the products
+      if (j + k >= n) v[t][k] = 0.f;
+      sum[k] += v[t][k];
     }
-    if (dz) {  // rows of dz are padded to 16 bytes
+    const int64_t i = i0 + t * 8;
+    if (dz && i < m && j < lddz) {  // lddz is a multiple of 8
       Vec8<T> o;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(v[k]);
-      T* row = dz + i * lddz + j;
-      if (j + 8 <= lddz) {
-        store8(row, o);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (j + k < lddz) row[k] = o.v[k];
-      }
+      for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(v[t][k]);
+      store8(dz + i * lddz + j, o);
     }
   }
   if (!partials) return;
@@ -192,14 +198,8 @@ __global__ __launch_bounds__(256) void act_bwd_k(
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void fold_bias_k(const float* partials,
-                                                   int64_t chunks, int64_t n,
-                                                   T* dbias) {
-  const int64_t j = global_tid();
-  if (j >= n) return;
-  double sum = 0.0;  // as many chunks as there are rows / 32
-  for (int64_t c = 0; c < chunks; ++c) sum += partials[c * n + j];
-  dbias[j] = from_f32<T>((float)sum);
+__global__ __launch_bounds__(256) void fold_bias_k(DdlBiasFold f) {
+  fold_bias<T>(f, global_tid());
 }
 
 // ---- rows that do not begin or end at 16 bytes -------------------------------
@@ -236,27 +236,20 @@ __global__ __launch_bounds__(256) void pack_rows_k(PackArgs a) {
 template <typename T, typename Z>
 void run_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz,
                  void* dz, int64_t lddz, int64_t m, int64_t n, int act,
-                 float* partials, void* dbias, hipStream_t s) {
-  const int64_t chunks = cdiv(m, BWD_ROWS);
-  const unsigned blocks = (unsigned)(chunks * cdiv(n, BWD_COLS));
-  const int wide =
-      (lddy % (16 / (int)sizeof(T)) == 0 && takes16(dy) ? 1 : 0) |
-      (ldz % (16 / (int)sizeof(Z)) == 0 && takes16(z) ? 2 : 0);
-  act_bwd_k<T, Z><<<blocks, 256, 0, s>>>(
-      (const T*)dy, lddy, (const Z*)z, ldz, (T*)dz, lddz, m, n, act, wide,
-      dbias ? partials : nullptr);
-  if (dbias)
-    fold_bias_k<T><<<(unsigned)cdiv(n, 256), 256, 0, s>>>(partials, chunks, n,
-                                                          (T*)dbias);
+                 float* partials, hipStream_t s) {
+  const unsigned blocks =
+      (unsigned)(cdiv(m, BWD_ROWS) * cdiv(n, BWD_COLS));
+  act_bwd_k<T, Z><<<blocks, 256, 0, s>>>((const T*)dy, lddy, (const Z*)z, ldz,
+                                         (T*)dz, lddz, m, n, act, partials);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t ddl_product_ws_floats(const DdlProduct* p) {
-  const Plan plan = plan_of(p);
-  return plan.splits > 1 ? plan.splits * p->m * cdiv(p->n, 8) * 8 : 0;
+int64_t ddl_product_plan(DdlProduct* p) {
+  plan_product(p);
+  return p->splits > 1 ? p->splits * p->m * cdiv(p->n, 8) * 8 : 0;
 }
 
 void ddl_product(const DdlProduct* p, hipStream_t s) {
@@ -264,6 +257,19 @@ void ddl_product(const DdlProduct* p, hipStream_t s) {
     case 0: ddl_product_f32(p, s); break;
     case 1: ddl_product_bf16(p, s); break;
     case 2: ddl_product_f16(p, s); break;
+  }
+}
+
+bool ddl_small_backward(const DdlProduct* dx, const DdlProduct* dw) {
+  return small_backward(dx, dw);
+}
+
+void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
+                        const DdlBiasFold* bias, hipStream_t s) {
+  switch (dx->dtype) {
+    case 0: ddl_backward_small_f32(dx, dw, bias, s); break;
+    case 1: ddl_backward_small_bf16(dx, dw, bias, s); break;
+    case 2: ddl_backward_small_f16(dx, dw, bias, s); break;
   }
 }
 
@@ -277,36 +283,30 @@ void ddl_product_few(const DdlProduct* p, hipStream_t s) {
   }
 }
 
-int64_t ddl_act_bwd_ws_floats(int64_t m, int64_t n) {
-  return cdiv(m, BWD_ROWS) * n;
-}
+int64_t ddl_bias_chunks(int64_t m) { return cdiv(m, BWD_ROWS); }
 
 void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
                  int64_t ldz, void* dz, int64_t lddz, int64_t m, int64_t n,
-                 int act, int dtype, float* partials, void* dbias,
-                 hipStream_t s) {
+                 int act, int dtype, float* partials, hipStream_t s) {
+#define RUN(T, Z) \
+  run_act_bwd<T, Z>(dy, lddy, z, ldz, dz, lddz, m, n, act, partials, s)
   switch (dtype * 2 + (z_f32 ? 1 : 0)) {
     case 0:
-    case 1:
-      run_act_bwd<float, float>(dy, lddy, z, ldz, dz, lddz, m, n, act,
-                                partials, dbias, s);
-      break;
-    case 2:
-      run_act_bwd<bf16, bf16>(dy, lddy, z, ldz, dz, lddz, m, n, act, partials,
-                              dbias, s);
-      break;
-    case 3:
-      run_act_bwd<bf16, float>(dy, lddy, z, ldz, dz, lddz, m, n, act,
-                               partials, dbias, s);
-      break;
-    case 4:
-      run_act_bwd<f16, f16>(dy, lddy, z, ldz, dz, lddz, m, n, act, partials,
-                            dbias, s);
-      break;
-    case 5:
-      run_act_bwd<f16, float>(dy, lddy, z, ldz, dz, lddz, m, n, act, partials,
-                              dbias, s);
-      break;
+    case 1: RUN(float, float); break;
+    case 2: RUN(bf16, bf16); break;
+    case 3: RUN(bf16, float); break;
+    case 4: RUN(f16, f16); break;
+    case 5: RUN(f16, float); break;
+  }
+#undef RUN
+}
+
+void ddl_fold_bias(const DdlBiasFold* f, int dtype, hipStream_t s) {
+  const unsigned blocks = (unsigned)cdiv(f->n, 256);
+  switch (dtype) {
+    case 0: fold_bias_k<float><<<blocks, 256, 0, s>>>(*f); break;
+    case 1: fold_bias_k<bf16><<<blocks, 256, 0, s>>>(*f); break;
+    case 2: fold_bias_k<f16><<<blocks, 256, 0, s>>>(*f); break;
   }
 }
 

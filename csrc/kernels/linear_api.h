@@ -27,10 +27,15 @@ struct DdlProduct {
   float* z;             // [m][ldo], or null
   int act;
   int dtype;
-  float* slabs;         // ddl_product_ws_floats floats
+  // filled in by ddl_product_plan
+  int side, splits;
+  float us;             // its estimate
+  int64_t steps, steps_per_split;
+  float* slabs;         // as many floats as the plan says
 };
 
-int64_t ddl_product_ws_floats(const DdlProduct* p);
+// Chooses tile and split; returns the floats that slabs has to hold.
+int64_t ddl_product_plan(DdlProduct* p);
 void ddl_product(const DdlProduct* p, hipStream_t s);
 
 // The same for at most ddl_few_rows() rows, both operands with r contiguous
@@ -38,15 +43,28 @@ void ddl_product(const DdlProduct* p, hipStream_t s);
 int ddl_few_rows(void);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
-// dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz, and the column
-// sums of dz before its rounding: partial sums (ddl_act_bwd_ws_floats floats),
-// then their fold into dbias.  z is float32 (z_f32), or for act 1 the output
-// in the tensors' dtype.  dz or dbias may be null.
-int64_t ddl_act_bwd_ws_floats(int64_t m, int64_t n);
+// dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of
+// 8), and the column sums of dz before its rounding, of 32 rows each: partials
+// holds ddl_bias_chunks(m) * n floats.  z is float32 (z_f32), or for act 1 the
+// output in the tensors' dtype.  dz or partials may be null.
+int64_t ddl_bias_chunks(int64_t m);
 void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
                  int64_t ldz, void* dz, int64_t lddz, int64_t m, int64_t n,
-                 int act, int dtype, float* partials, void* dbias,
-                 hipStream_t s);
+                 int act, int dtype, float* partials, hipStream_t s);
+
+// dbias[j] = sum of partials[c][j]; nothing for n = 0.
+struct DdlBiasFold {
+  const float* partials;
+  void* dbias;
+  int64_t chunks, n;
+};
+void ddl_fold_bias(const DdlBiasFold* f, int dtype, hipStream_t s);
+
+// dx and dw, planned, and the fold in one launch, where that is estimated to
+// be faster than a launch each.
+bool ddl_small_backward(const DdlProduct* dx, const DdlProduct* dw);
+void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
+                        const DdlBiasFold* bias, hipStream_t s);
 
 // dst[i][0..ldd) = src[i][0..n), then zeros, for one or two matrices; ldd is a
 // multiple of 8, dst of 16 bytes.

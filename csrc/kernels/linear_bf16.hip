@@ -5,3 +5,8 @@
 void ddl_product_bf16(const DdlProduct* p, hipStream_t s) {
   run_product<bf16>(p, s);
 }
+
+void ddl_backward_small_bf16(const DdlProduct* dx, const DdlProduct* dw,
+                           const DdlBiasFold* bias, hipStream_t s) {
+  run_backward_small<bf16>(*dx, *dw, *bias, s);
+}

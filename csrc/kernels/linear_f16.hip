@@ -5,3 +5,8 @@
 void ddl_product_f16(const DdlProduct* p, hipStream_t s) {
   run_product<f16>(p, s);
 }
+
+void ddl_backward_small_f16(const DdlProduct* dx, const DdlProduct* dw,
+                           const DdlBiasFold* bias, hipStream_t s) {
+  run_backward_small<f16>(*dx, *dw, *bias, s);
+}

@@ -28,6 +28,7 @@
 #include "common.h"
 #include "linear_api.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -49,7 +50,6 @@ struct Epilogue {
   float* z;
   int64_t ldo, ldres, m, n;
   int act;
-  int wide;  // rows of out, z and residual take 16-byte accesses
 };
 
 struct Product {
@@ -144,6 +144,21 @@ __device__ __forceinline__ void activate8(float* y, int act) {
   }
 }
 
+// v[k] *= act'(z[k])
+__device__ __forceinline__ void activate_grad8(float* v, const float* z,
+                                               int act) {
+  auto all = [&](auto which) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= activate_grad(z[k], which.value);
+  };
+  switch (act) {
+    case 1: all(std::integral_constant<int, 1>{}); break;
+    case 2: all(std::integral_constant<int, 2>{}); break;
+    case 3: all(std::integral_constant<int, 3>{}); break;
+    case 4: all(std::integral_constant<int, 4>{}); break;
+  }
+}
+
 // Columns j..j+7 of row i; `sum` is the product.
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t i,
@@ -157,22 +172,19 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t i,
   float* zout = e.z ? e.z + i * e.ldo + j : nullptr;
   const T* res =
       e.residual ? (const T*)e.residual + i * e.ldres + j : nullptr;
-  if (e.wide && j + 8 <= e.n) {
-    Vec8<T> o;
+  if (j + 8 <= e.n) {
+    // rows begin anywhere: 16-byte accesses do not need their alignment
+    T o[8];
     if (res) {
-      const Vec8<T> r = load8(res);
+      T r[8];
+      __builtin_memcpy(r, res, sizeof(r));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] += to_f32(r.v[k]);
+      for (int k = 0; k < 8; ++k) y[k] += to_f32(r[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(y[k]);
-    store8(out, o);
-    if (zout) {
-      Vec8<float> q;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) q.v[k] = z[k];
-      store8(zout, q);
-    }
+    for (int k = 0; k < 8; ++k) o[k] = from_f32<T>(y[k]);
+    __builtin_memcpy(out, o, sizeof(o));
+    if (zout) __builtin_memcpy(zout, z, sizeof(z));
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -192,15 +204,9 @@ __device__ __forceinline__ void load_bias8(const Epilogue& e, int64_t j,
     bias[k] = e.bias && j + k < e.n ? to_f32(((const T*)e.bias)[j + k]) : 0.f;
 }
 
-template <typename T> Epilogue epilogue_of(const DdlProduct* d) {
-  const int64_t per = 16 / (int)sizeof(T);
-  auto wide = [&](const void* p, int64_t ld) {
-    return ((uintptr_t)p & 15) == 0 && ld % per == 0;
-  };
-  return Epilogue{d->bias, d->residual, d->out, d->z, d->ldo, d->ldres, d->m,
-                  d->n, d->act,
-                  wide(d->out, d->ldo) &&
-                      (!d->residual || wide(d->residual, d->ldres))};
+inline Epilogue epilogue_of(const DdlProduct* d) {
+  return Epilogue{d->bias, d->residual, d->out, d->z, d->ldo,
+                  d->ldres, d->m, d->n, d->act};
 }
 
 // ---- the tiled product -----------------------------------------------------
@@ -391,21 +397,24 @@ __device__ __forceinline__ void write_out(const Product& p, char* smem,
   }
 }
 
+template <typename T, int BM, int BN, int STAGES>
+constexpr int lds_bytes() { return STAGES * (BM + BN) * LINE; }
+
+// Block `id` of the product, with lds_bytes of LDS.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_COL,
           bool B_COL>
-__global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
+__device__ __forceinline__ void product_block(const Product& p, unsigned id,
+                                              char* smem) {
   constexpr int WAVES = WM * WN;
   constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   static_assert(NI % 4 == 0, "a lane's 16 columns are 4 fragments");
   using TA = Tile<T, A_COL, false, BM, WAVES>;
   using TB = Tile<T, B_COL, true, BN, WAVES>;
   constexpr int STAGE = TA::BYTES + TB::BYTES;
-  __shared__ __align__(16) char smem[STAGES * STAGE];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = p.tiles_m * p.tiles_n;
-  const unsigned id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int split = id / tiles;
   const int tile = id % tiles;
   // i runs fastest: neighbours on an XCD share the b tile
@@ -502,6 +511,42 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
                                               i0 + wm, j0 + wn);
 }
 
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_COL,
+          bool B_COL>
+__global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
+  __shared__ __align__(16) char smem[lds_bytes<T, BM, BN, STAGES>()];
+  product_block<T, BM, BN, WM, WN, STAGES, A_COL, B_COL>(
+      p, xcd_swizzle(blockIdx.x, gridDim.x), smem);
+}
+
+// Column j of the bias gradient: the fold of act_bwd_k's partial sums.
+template <typename T>
+__device__ __forceinline__ void fold_bias(const DdlBiasFold& f,
+                                          int64_t j) {
+  if (j >= f.n) return;
+  double sum = 0.0;  // as many chunks as there are rows / 32
+  for (int64_t c = 0; c < f.chunks; ++c) sum += f.partials[c * f.n + j];
+  ((T*)f.dbias)[j] = from_f32<T>((float)sum);
+}
+
+// Both products of a small layer's backward pass and the fold of its bias
+// gradient, side by side in one launch: each alone leaves most of the GPU
+// idle, and a launch costs the host 4 us.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void backward_small_k(
+    Product dx, Product dw, DdlBiasFold bias) {
+  __shared__ __align__(16) char smem[lds_bytes<T, 64, 64, 4>()];
+  unsigned id = blockIdx.x;
+  const unsigned nx = dx.tiles_m * dx.tiles_n, nw = dw.tiles_m * dw.tiles_n;
+  if (id < nx) {
+    product_block<T, 64, 64, 4, 1, 4, false, true>(dx, id, smem);
+  } else if (id < nx + nw) {
+    product_block<T, 64, 64, 4, 1, 4, true, true>(dw, id - nx, smem);
+  } else {
+    fold_bias<T>(bias, (int64_t)(id - nx - nw) * 256 + threadIdx.x);
+  }
+}
+
 // Adds the slabs in order (no atomics: the result does not depend on which
 // block ends first) and applies the epilogue; 8 columns a thread.
 template <typename T>
@@ -536,8 +581,6 @@ inline int compute_units() {
   return n;
 }
 
-inline bool takes16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 // Tile sizes, blocks a compute unit holds, and measured times in us: of a
 // step (128 bytes of r) where a unit holds one block and where it is full,
 // and of a block's beginning and end.
@@ -557,37 +600,29 @@ constexpr TileKind KINDS16[] = {{256, 1, 1.2f, 1.5f, 7.f},
 constexpr TileKind KINDS32[] = {{128, 2, 2.0f, 3.8f, 3.f},
                                 {64, 2, 0.6f, 1.1f, 1.5f}};
 
-struct Plan {
-  TileKind kind;
-  int splits;
-  int64_t steps, steps_per_split;
-};
-
 // The tile and the split of r with the smallest estimate: rounds of blocks
 // over the compute units, and for a split the launch that joins its slabs
 // (4 us and their bytes, written and read, at 10 TB/s: they stay in the last
 // level cache).
-inline Plan plan_of(const DdlProduct* p) {
-  const int size = p->dtype == 0 ? 4 : 2;
-  const int64_t steps = cdiv(p->r * size, LINE);
-  Plan best{};
-  float best_us = 0.f;
+inline void plan_product(DdlProduct* p) {
+  constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  const float units = (float)compute_units();
+  p->steps = cdiv(p->r * (p->dtype == 0 ? 4 : 2), LINE);
+  p->side = 0;
   auto consider = [&](const TileKind& k) {
-    const int64_t tiles = cdiv(p->m, k.side) * cdiv(p->n, k.side);
-    for (int64_t s = 1; s <= 32; ++s) {
-      if (s > 1 && steps < 2 * s) break;
-      const int64_t per = std::max<int64_t>(1, cdiv(steps, s));
-      const int64_t splits = std::max<int64_t>(1, cdiv(steps, per));
-      if (splits != s) continue;
-      const int64_t blocks = tiles * splits;
-      const int64_t rounds =
-          cdiv(blocks, (int64_t)compute_units() * k.per_unit);
-      const float step = blocks <= compute_units() ? k.alone : k.full;
-      float us = rounds * (k.ends + per * step);
-      if (splits > 1) us += 4.f + splits * p->m * p->n * 8e-7f;
-      if (best.kind.side == 0 || us < best_us) {
-        best_us = us;
-        best = Plan{k, (int)splits, steps, per};
+    const float tiles = (float)(cdiv(p->m, k.side) * cdiv(p->n, k.side));
+    for (const int s : SPLITS) {
+      if (s > 1 && p->steps < 2 * s) break;
+      const float per = std::ceil((float)p->steps / s);
+      const float blocks = tiles * s;
+      const float step = blocks <= units ? k.alone : k.full;
+      float us = std::ceil(blocks / (units * k.per_unit)) *
+                 (k.ends + per * step);
+      if (s > 1) us += 4.f + s * (float)p->m * (float)p->n * 8e-7f;
+      if (p->side == 0 || us < p->us) {
+        p->us = us;
+        p->side = k.side;
+        p->splits = s;
       }
     }
   };
@@ -595,7 +630,41 @@ inline Plan plan_of(const DdlProduct* p) {
     for (const auto& k : KINDS32) consider(k);
   else
     for (const auto& k : KINDS16) consider(k);
-  return best;
+  p->steps_per_split = std::max<int64_t>(1, cdiv(p->steps, p->splits));
+  p->splits = (int)std::max<int64_t>(1, cdiv(p->steps, p->steps_per_split));
+}
+
+// Whether dx and dw, both planned, are better off in backward_small_k: its
+// blocks go through the units two at a time, and the longest one is waited
+// for; a launch of their own costs each 4 us.
+inline bool small_backward(const DdlProduct* dx, const DdlProduct* dw) {
+  const TileKind k = dx->dtype == 0 ? KINDS32[1] : KINDS16[2];
+  float work = 0.f, longest = 0.f;
+  for (const auto* p : {dx, dw}) {
+    const float tiles = (float)(cdiv(p->m, k.side) * cdiv(p->n, k.side));
+    work += tiles * (k.ends + p->steps * k.full);
+    longest = std::max(longest, k.ends + p->steps * k.alone);
+  }
+  return std::max(work / (compute_units() * k.per_unit), longest) <
+         dx->us + dw->us + 4.f;
+}
+
+template <typename T> Product product_of(const DdlProduct* d) {
+  Product p{};
+  p.a = (const char*)d->a;
+  p.b = (const char*)d->b;
+  p.lda = d->lda * (int64_t)sizeof(T);
+  p.ldb = d->ldb * (int64_t)sizeof(T);
+  p.r = d->r;
+  p.steps = d->steps;
+  p.steps_per_split = d->steps_per_split;
+  p.splits = d->splits;
+  p.tiles_m = (int)cdiv(d->m, d->side);
+  p.tiles_n = (int)cdiv(d->n, d->side);
+  p.slabs = d->slabs;
+  p.ldslab = cdiv(d->n, 8) * 8;
+  p.e = epilogue_of(d);
+  return p;
 }
 
 template <typename T, int SIDE, int WM, int WN, int STAGES>
@@ -614,25 +683,11 @@ void launch_product(const Product& p, int a_col, int b_col, hipStream_t s) {
 
 template <typename T>
 void run_product(const DdlProduct* d, hipStream_t s) {
-  const Plan plan = plan_of(d);
-  Product p{};
-  p.a = (const char*)d->a;
-  p.b = (const char*)d->b;
-  p.lda = d->lda * (int64_t)sizeof(T);
-  p.ldb = d->ldb * (int64_t)sizeof(T);
-  p.r = d->r;
-  p.steps = plan.steps;
-  p.steps_per_split = plan.steps_per_split;
-  p.splits = plan.splits;
-  p.tiles_m = (int)cdiv(d->m, plan.kind.side);
-  p.tiles_n = (int)cdiv(d->n, plan.kind.side);
-  p.slabs = d->slabs;
-  p.ldslab = cdiv(d->n, 8) * 8;
-  p.e = epilogue_of<T>(d);
-  if (plan.kind.side == 256) {
+  const Product p = product_of<T>(d);
+  if (d->side == 256) {
     if constexpr (sizeof(T) == 2)
       launch_product<T, 256, 2, 4, 2>(p, d->a_col, d->b_col, s);
-  } else if (plan.kind.side == 128) {
+  } else if (d->side == 128) {
     launch_product<T, 128, 2, 2, 2>(p, d->a_col, d->b_col, s);
   } else {
     launch_product<T, 64, 4, 1, 4>(p, d->a_col, d->b_col, s);
@@ -642,6 +697,20 @@ void run_product(const DdlProduct* d, hipStream_t s) {
     join_k<T><<<(unsigned)cdiv(threads, 256), 256, 0, s>>>(
         p.slabs, p.splits, p.ldslab, p.e);
   }
+}
+
+template <typename T>
+void run_backward_small(DdlProduct dx, DdlProduct dw, const DdlBiasFold& bias,
+                        hipStream_t s) {
+  for (auto* p : {&dx, &dw}) {
+    p->side = 64;
+    p->splits = 1;
+    p->steps_per_split = std::max<int64_t>(1, p->steps);
+  }
+  const Product x = product_of<T>(&dx), w = product_of<T>(&dw);
+  const int64_t blocks = (int64_t)x.tiles_m * x.tiles_n +
+                         (int64_t)w.tiles_m * w.tiles_n + cdiv(bias.n, 256);
+  backward_small_k<T><<<(unsigned)blocks, 256, 0, s>>>(x, w, bias);
 }
 
 }  // namespace
