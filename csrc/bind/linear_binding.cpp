@@ -344,8 +344,21 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
   return matrix ? y : y.view(shape);
 }
 
+// (bm, bn, stages, parts of r) that a product of this size takes.
+std::tuple<int, int, int, int> linear_plan(int64_t m, int64_t n, int64_t r,
+                                           int dtype) {
+  DdlProduct p{};
+  p.m = m;
+  p.n = n;
+  p.r = r;
+  p.dtype = dtype;
+  ddl_product_plan(&p);
+  return {p.bm, p.bn, p.stages, p.splits};
+}
+
 }  // namespace
 
 void bind_linear(pybind11::module& m) {
   m.def("linear_act", &linear_act);
+  m.def("linear_plan", &linear_plan);
 }

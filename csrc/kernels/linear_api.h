@@ -28,7 +28,7 @@ struct DdlProduct {
   int act;
   int dtype;
   // filled in by ddl_product_plan
-  int side, splits;
+  int kind, bm, bn, stages, splits;
   float us;             // its estimate
   int64_t steps, steps_per_split;
   float* slabs;         // as many floats as the plan says

@@ -525,6 +525,7 @@ __device__ __forceinline__ void fold_bias(const DdlBiasFold& f,
                                           int64_t j) {
   if (j >= f.n) return;
   double sum = 0.0;  // as many chunks as there are rows / 32
+#pragma unroll 8
   for (int64_t c = 0; c < f.chunks; ++c) sum += f.partials[c * f.n + j];
   ((T*)f.dbias)[j] = from_f32<T>((float)sum);
 }
@@ -558,12 +559,13 @@ __global__ __launch_bounds__(256) void join_k(const float* slabs, int splits,
   const int64_t i = at / groups, j = (at % groups) * 8;
   if (j >= e.n) return;
   float sum[8] = {};
+  const float* first = slabs + i * ldslab + j;
+  const int64_t slab = e.m * ldslab;
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
-    const float* q = slabs + (s * e.m + i) * ldslab + j;
-    const float4 lo = *reinterpret_cast<const float4*>(q);
-    const float4 hi = *reinterpret_cast<const float4*>(q + 4);
-    sum[0] += lo.x; sum[1] += lo.y; sum[2] += lo.z; sum[3] += lo.w;
-    sum[4] += hi.x; sum[5] += hi.y; sum[6] += hi.z; sum[7] += hi.w;
+    const Vec8<float> q = load8(first + s * slab);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += q.v[k];
   }
   float bias[8];
   load_bias8<T>(e, j, bias);
@@ -581,55 +583,70 @@ inline int compute_units() {
   return n;
 }
 
-// Tile sizes, blocks a compute unit holds, and measured times in us: of a
-// step (128 bytes of r) where a unit holds one block and where it is full,
-// and of a block's beginning and end.
+// A tile of bm x bn, blocks a compute unit holds, and measured times in us: of
+// a step (128 bytes of r) where half of the room is taken and where all is, and
+// of a block's beginning and end.
 struct TileKind {
-  int side, per_unit;
+  int bm, bn, stages, per_unit;
   float alone, full, ends;
 };
 
-// bf16 and f16.  4096^3, forward / dx / dW: 256 takes 104 / 103 / 107 us, 128
-// 122 / 134 / 152, 64 307 / 300 / 301; 256 x 2048 x 1000 split for each: 64
-// takes 11 / 10 / 7, 128 13 / 14 / 9, 256 16 and more.
-constexpr TileKind KINDS16[] = {{256, 1, 1.2f, 1.5f, 7.f},
-                                {128, 2, 0.68f, 0.95f, 3.f},
-                                {64, 2, 0.23f, 0.6f, 1.5f}};
-// float32: 4096^3 980 (128) against 1127 (64); 256 x 2048 x 1000 19 (64)
-// against 26.
-constexpr TileKind KINDS32[] = {{128, 2, 2.0f, 3.8f, 3.f},
-                                {64, 2, 0.6f, 1.1f, 1.5f}};
+// bf16 and f16.  Each is fastest somewhere (us, the kernel alone; next best):
+//   256 x 256     4096^3 104, 128 x 128 122; dx of 512 x 25088 -> 4096 94, 120
+//   256 x 128     its forward, split in four, 97, 256 x 256 in eight 100
+//   128 x 128, 4  2048^3 24, 128 x 64 27; 1024 x 4096 -> 4096 42, 45
+//   128 x 128, 2  dW of 256 x 25088 -> 4096 93, 256 x 256 121
+//   128 x 64      512 x 4096 -> 4096 29, 64 x 64 31
+//   64 x 64       512^3 6.2, 128 x 64 7.5
+constexpr TileKind KINDS16[] = {{256, 256, 2, 1, 1.25f, 1.6f, 12.f},
+                                {256, 128, 3, 1, 0.8f, 0.88f, 9.f},
+                                {128, 128, 4, 1, 0.45f, 0.54f, 6.f},
+                                {128, 128, 2, 2, 0.75f, 1.f, 5.f},
+                                {128, 64, 3, 2, 0.39f, 0.64f, 4.5f},
+                                {64, 64, 4, 2, 0.27f, 0.45f, 3.f}};
+// float32: 4096^3 980 (128 x 128), 1016, 1127; dx of 512 x 25088 -> 4096 977,
+// 934 (128 x 64), 968; 256 x 2048 -> 1000 26, 21, 19 (64 x 64).
+constexpr TileKind KINDS32[] = {{128, 128, 2, 2, 2.f, 3.75f, 5.f},
+                                {128, 64, 3, 2, 1.05f, 2.f, 5.f},
+                                {64, 64, 4, 2, 0.64f, 1.1f, 4.f}};
 
 // The tile and the split of r with the smallest estimate: rounds of blocks
 // over the compute units, and for a split the launch that joins its slabs
-// (4 us and their bytes, written and read, at 10 TB/s: they stay in the last
-// level cache).
+// (3 us and 0.2 us a MB of them).
 inline void plan_product(DdlProduct* p) {
   constexpr int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
   const float units = (float)compute_units();
   p->steps = cdiv(p->r * (p->dtype == 0 ? 4 : 2), LINE);
-  p->side = 0;
-  auto consider = [&](const TileKind& k) {
-    const float tiles = (float)(cdiv(p->m, k.side) * cdiv(p->n, k.side));
+  p->kind = -1;
+  auto consider = [&](const TileKind& k, int kind) {
+    const float tiles = (float)(cdiv(p->m, k.bm) * cdiv(p->n, k.bn));
     for (const int s : SPLITS) {
       if (s > 1 && p->steps < 2 * s) break;
       const float per = std::ceil((float)p->steps / s);
       const float blocks = tiles * s;
-      const float step = blocks <= units ? k.alone : k.full;
-      float us = std::ceil(blocks / (units * k.per_unit)) *
-                 (k.ends + per * step);
-      if (s > 1) us += 4.f + s * (float)p->m * (float)p->n * 8e-7f;
-      if (p->side == 0 || us < p->us) {
+      float rounds = blocks / (units * k.per_unit);
+      // up to half of the units' room, then towards all of it
+      const float share = std::min(std::max(2.f * rounds - 1.f, 0.f), 1.f);
+      const float step = k.alone + share * (k.full - k.alone);
+      // many rounds do not end together
+      rounds = rounds <= 3.f ? std::ceil(rounds) : rounds + 0.5f;
+      float us = rounds * (k.ends + per * step);
+      if (s > 1) us += 3.f + s * (float)p->m * (float)p->n * 8e-7f;
+      if (p->kind < 0 || us < p->us) {
         p->us = us;
-        p->side = k.side;
+        p->kind = kind;
+        p->bm = k.bm;
+        p->bn = k.bn;
+        p->stages = k.stages;
         p->splits = s;
       }
     }
   };
+  int kind = 0;
   if (p->dtype == 0)
-    for (const auto& k : KINDS32) consider(k);
+    for (const auto& k : KINDS32) consider(k, kind++);
   else
-    for (const auto& k : KINDS16) consider(k);
+    for (const auto& k : KINDS16) consider(k, kind++);
   p->steps_per_split = std::max<int64_t>(1, cdiv(p->steps, p->splits));
   p->splits = (int)std::max<int64_t>(1, cdiv(p->steps, p->steps_per_split));
 }
@@ -638,10 +655,10 @@ inline void plan_product(DdlProduct* p) {
 // blocks go through the units two at a time, and the longest one is waited
 // for; a launch of their own costs each 4 us.
 inline bool small_backward(const DdlProduct* dx, const DdlProduct* dw) {
-  const TileKind k = dx->dtype == 0 ? KINDS32[1] : KINDS16[2];
+  const TileKind k = dx->dtype == 0 ? KINDS32[2] : KINDS16[5];
   float work = 0.f, longest = 0.f;
   for (const auto* p : {dx, dw}) {
-    const float tiles = (float)(cdiv(p->m, k.side) * cdiv(p->n, k.side));
+    const float tiles = (float)(cdiv(p->m, k.bm) * cdiv(p->n, k.bn));
     work += tiles * (k.ends + p->steps * k.full);
     longest = std::max(longest, k.ends + p->steps * k.alone);
   }
@@ -659,38 +676,63 @@ template <typename T> Product product_of(const DdlProduct* d) {
   p.steps = d->steps;
   p.steps_per_split = d->steps_per_split;
   p.splits = d->splits;
-  p.tiles_m = (int)cdiv(d->m, d->side);
-  p.tiles_n = (int)cdiv(d->n, d->side);
+  p.tiles_m = (int)cdiv(d->m, d->bm);
+  p.tiles_n = (int)cdiv(d->n, d->bn);
   p.slabs = d->slabs;
   p.ldslab = cdiv(d->n, 8) * 8;
   p.e = epilogue_of(d);
   return p;
 }
 
-template <typename T, int SIDE, int WM, int WN, int STAGES>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 void launch_product(const Product& p, int a_col, int b_col, hipStream_t s) {
   const dim3 grid(p.tiles_m * p.tiles_n * p.splits), block(WM * WN * 64);
   if (a_col && b_col)
-    product_k<T, SIDE, SIDE, WM, WN, STAGES, true, true>
-        <<<grid, block, 0, s>>>(p);
+    product_k<T, BM, BN, WM, WN, STAGES, true, true><<<grid, block, 0, s>>>(p);
   else if (b_col)
-    product_k<T, SIDE, SIDE, WM, WN, STAGES, false, true>
+    product_k<T, BM, BN, WM, WN, STAGES, false, true>
         <<<grid, block, 0, s>>>(p);
   else
-    product_k<T, SIDE, SIDE, WM, WN, STAGES, false, false>
+    product_k<T, BM, BN, WM, WN, STAGES, false, false>
         <<<grid, block, 0, s>>>(p);
 }
 
 template <typename T>
 void run_product(const DdlProduct* d, hipStream_t s) {
   const Product p = product_of<T>(d);
-  if (d->side == 256) {
-    if constexpr (sizeof(T) == 2)
-      launch_product<T, 256, 2, 4, 2>(p, d->a_col, d->b_col, s);
-  } else if (d->side == 128) {
-    launch_product<T, 128, 2, 2, 2>(p, d->a_col, d->b_col, s);
+  if constexpr (sizeof(T) == 2) {
+    switch (d->kind) {
+      case 0:
+        launch_product<T, 256, 256, 2, 4, 2>(p, d->a_col, d->b_col, s);
+        break;
+      case 1:
+        launch_product<T, 256, 128, 4, 2, 3>(p, d->a_col, d->b_col, s);
+        break;
+      case 2:
+        launch_product<T, 128, 128, 4, 2, 4>(p, d->a_col, d->b_col, s);
+        break;
+      case 3:
+        launch_product<T, 128, 128, 4, 2, 2>(p, d->a_col, d->b_col, s);
+        break;
+      case 4:
+        launch_product<T, 128, 64, 4, 1, 3>(p, d->a_col, d->b_col, s);
+        break;
+      case 5:
+        launch_product<T, 64, 64, 4, 1, 4>(p, d->a_col, d->b_col, s);
+        break;
+    }
   } else {
-    launch_product<T, 64, 4, 1, 4>(p, d->a_col, d->b_col, s);
+    switch (d->kind) {
+      case 0:
+        launch_product<T, 128, 128, 4, 2, 2>(p, d->a_col, d->b_col, s);
+        break;
+      case 1:
+        launch_product<T, 128, 64, 4, 1, 3>(p, d->a_col, d->b_col, s);
+        break;
+      case 2:
+        launch_product<T, 64, 64, 4, 1, 4>(p, d->a_col, d->b_col, s);
+        break;
+    }
   }
   if (p.splits > 1) {
     const int64_t threads = p.ldslab / 8 * d->m;
@@ -703,7 +745,8 @@ template <typename T>
 void run_backward_small(DdlProduct dx, DdlProduct dw, const DdlBiasFold& bias,
                         hipStream_t s) {
   for (auto* p : {&dx, &dw}) {
-    p->side = 64;
+    p->kind = sizeof(T) == 4 ? 2 : 5;
+    p->bm = p->bn = 64;
     p->splits = 1;
     p->steps_per_split = std::max<int64_t>(1, p->steps);
   }

@@ -15,6 +15,7 @@ import torch
 
 from distributeddeeplearning_amd import ops
 from distributeddeeplearning_amd.ops import functional as DF
+from distributeddeeplearning_amd.ops import load_kernels_ext
 
 U = torch.finfo(torch.float32).eps / 2
 gpu = pytest.mark.gpu
@@ -144,6 +145,49 @@ def test_epilogues(act, bias, residual, dtype, device):
                                    (1, 25088, 1000), (700, 30, 3000)])
 def test_larger(shape, dtype):
     run_case(*shape, dtype, "cuda", "gelu" if shape[0] % 2 else "relu")
+
+
+# sizes that reach every tile of the kernel in every product, and split ones
+PLANNED = {
+    torch.bfloat16: [(2056, 264, 4104), (2056, 4104, 136), (136, 4104, 2056),
+                     (1032, 72, 2056), (1032, 2056, 136), (72, 2056, 1032),
+                     (2056, 72, 2056), (2056, 2056, 136), (72, 2056, 2056),
+                     (2000, 2048, 2040), (136, 8200, 4104), (72, 1032, 136),
+                     (392, 16392, 2440), (1032, 16392, 2120)],
+    torch.float32: [(1032, 72, 2056), (1032, 2056, 136), (72, 2056, 1032),
+                    (2056, 72, 2056), (2056, 2056, 136), (72, 2056, 2056),
+                    (72, 4104, 4104), (72, 264, 136), (2056, 72, 4104)],
+}
+PLANNED[torch.float16] = PLANNED[torch.bfloat16]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,shape", [(d, s) for d in DTYPES
+                                         for s in PLANNED[d]])
+def test_every_tile(dtype, shape):
+    run_case(*shape, dtype, "cuda", "silu")
+
+
+def test_every_tile_is_planned():
+    ext = load_kernels_ext(required=False)
+    if ext is None:
+        pytest.skip("extension not built")
+    kinds16 = {(256, 256, 2), (256, 128, 3), (128, 128, 4), (128, 128, 2),
+               (128, 64, 3), (64, 64, 4)}
+    kinds32 = {(128, 128, 2), (128, 64, 3), (64, 64, 4)}
+    for dtype, code, kinds in ((torch.bfloat16, 1, kinds16),
+                               (torch.float32, 0, kinds32)):
+        seen, split = {"fwd": set(), "dx": set(), "dw": set()}, set()
+        for m, k, n in PLANNED[dtype]:
+            for name, size in (("fwd", (m, n, k)), ("dx", (m, k, n)),
+                               ("dw", (n, k, m))):
+                *kind, splits = ext.linear_plan(*size, code)
+                seen[name].add(tuple(kind))
+                split.add(splits > 1)
+        assert seen["fwd"] == kinds and seen["dx"] == kinds
+        # 256 x 128 takes dW of very many rows only; dx has the same b tile
+        assert seen["dw"] | {(256, 128, 3)} >= kinds
+        assert split == {True, False}
 
 
 def _offset(t):
