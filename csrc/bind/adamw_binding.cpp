@@ -5,7 +5,9 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
+#include <algorithm>
 #include <memory>
+#include <numeric>
 #include <unordered_set>
 #include <vector>
 
@@ -95,30 +97,31 @@ class AdamWPlan {
       }
       states_.push_back(std::move(s));
     }
-  }
-
-  // Places (in this plan) of parameters with a gradient and no state.
-  std::vector<int64_t> need() const {
-    std::vector<int64_t> out;
-    for (size_t i = 0; i < params_.size(); ++i)
-      if (params_[i].grad().defined() && !states_[i].step.defined())
-        out.push_back((int64_t)i);
-    return out;
+    // A launch takes so many tensors: the largest come first, so that all
+    // launches but one are short.
+    order_.resize(n);
+    std::iota(order_.begin(), order_.end(), 0);
+    std::stable_sort(order_.begin(), order_.end(), [&](int64_t a, int64_t b) {
+      return params_[a].numel() > params_[b].numel();
+    });
   }
 
   // Reads the gradients as they are now.  Those laid out unlike their
-  // parameter are copied into its layout first.
-  void collect() {
+  // parameter are copied into its layout first.  Returns the places (in this
+  // plan) of parameters with a gradient and no state.
+  std::vector<int64_t> collect() {
     c10::DeviceGuard guard(device_);
     rows_.clear();
     grads_.clear();
-    for (size_t i = 0; i < params_.size(); ++i) {
+    std::vector<int64_t> missing;
+    for (const int64_t i : order_) {
       const at::Tensor& p = params_[i];
-      at::Tensor g = p.grad();
-      if (!g.defined() || p.numel() == 0) continue;
+      const at::Tensor& grad = p.grad();
+      if (!grad.defined()) continue;
       const State& s = states_[i];
-      TORCH_CHECK(s.step.defined(), "parameter ", indices_[i],
-                  " has a gradient and no state");
+      if (!s.step.defined()) missing.push_back(i);
+      if (!s.step.defined() || p.numel() == 0) continue;
+      at::Tensor g = grad;
       check_grad(g);
       TORCH_CHECK(p.device() == device_ && p.scalar_type() == dtype_ &&
                       same_layout(p, s.m),
@@ -147,6 +150,7 @@ class AdamWPlan {
       rows_.push_back(r);
       grads_.push_back(std::move(g));
     }
+    return missing;
   }
 
   std::vector<DdlGradTensor> grad_rows() const {
@@ -157,23 +161,22 @@ class AdamWPlan {
   }
 
   // The update for what collect() saw; forgets the gradients afterwards.
-  void step(double lr, double beta1, double beta2, double eps,
-            double weight_decay, double grad_mul, int64_t seed,
-            const c10::optional<at::Tensor>& coef) {
-    if (!rows_.empty()) {
-      c10::DeviceGuard guard(device_);
-      const auto s = stream_now();
-      const int64_t n = (int64_t)rows_.size();
-      DdlAdamScalars c{lr, beta1, beta2, eps, weight_decay, (float)grad_mul,
-                       (uint32_t)seed};
+  void step(const DdlAdamScalars& c, const DdlNormFold* fold,
+            const float* coef) {
+    c10::DeviceGuard guard(device_);
+    const auto s = stream_now();
+    const int64_t n = (int64_t)rows_.size();
+    if (n) {
       at::Tensor ws = at::empty(
           {ddl_adamw_ws_bytes(n)},
           at::TensorOptions().dtype(at::kByte).device(device_));
-      ddl_adamw_prepare(rows_.data(), n, &c, ws.data_ptr(), s);
+      ddl_adamw_prepare(rows_.data(), n, &c, ws.data_ptr(), fold, s);
       ddl_adamw(rows_.data(), n, &c, code_of(dtype_), bits_, ws.data_ptr(),
-                coef.has_value() ? coef->const_data_ptr<float>() : nullptr, s);
-      C10_HIP_KERNEL_LAUNCH_CHECK();
+                coef, s);
+    } else if (fold) {
+      ddl_grad_norm_fold(fold, s);
     }
+    C10_HIP_KERNEL_LAUNCH_CHECK();
     rows_.clear();
     grads_.clear();
   }
@@ -215,6 +218,7 @@ class AdamWPlan {
   c10::Device device_{c10::kCPU};
   at::ScalarType dtype_;
   std::vector<State> states_;
+  std::vector<int64_t> order_;  // places, the largest parameter first
   std::vector<DdlAdamTensor> rows_;
   Tensors grads_;
 };
@@ -224,56 +228,83 @@ struct NormList {
   int dtype;
 };
 
-// norm (0-dim float32) and the clipping coefficient for these lists.
-std::tuple<at::Tensor, at::Tensor> norm_of(const std::vector<NormList>& lists,
-                                           c10::Device device, double mul,
-                                           double max_norm) {
+// Partial sums of these lists, and where norm and coefficient go (0-dim
+// float32 tensors); the fold is still to be launched.
+struct Norm {
+  at::Tensor partials, norm, coef;
+  DdlNormFold fold;
+};
+
+Norm norm_of(const std::vector<NormList>& lists, c10::Device device,
+             double mul, double max_norm) {
   const auto s = stream_now();
   const auto opts = at::TensorOptions().device(device);
+  Norm out;
   int64_t blocks = 0;
   for (const auto& l : lists)
     blocks += ddl_grad_norm_blocks(l.rows.data(), (int64_t)l.rows.size());
-  auto partials = at::empty({std::max<int64_t>(blocks, 1)},
-                            opts.dtype(at::kDouble));
-  auto norm = at::empty({}, opts.dtype(at::kFloat));
-  auto coef = at::empty({}, opts.dtype(at::kFloat));
-  double* out = partials.data_ptr<double>();
+  out.partials =
+      at::empty({std::max<int64_t>(blocks, 1)}, opts.dtype(at::kDouble));
+  out.norm = at::empty({}, opts.dtype(at::kFloat));
+  out.coef = at::empty({}, opts.dtype(at::kFloat));
+  double* at = out.partials.data_ptr<double>();
   for (const auto& l : lists) {
     const int64_t n = (int64_t)l.rows.size();
-    ddl_grad_norm_partials(l.rows.data(), n, l.dtype, out, s);
-    out += ddl_grad_norm_blocks(l.rows.data(), n);
+    ddl_grad_norm_partials(l.rows.data(), n, l.dtype, at, s);
+    at += ddl_grad_norm_blocks(l.rows.data(), n);
   }
-  ddl_grad_norm_finish(partials.data_ptr<double>(), blocks, mul, max_norm,
-                       norm.data_ptr<float>(), coef.data_ptr<float>(), s);
-  C10_HIP_KERNEL_LAUNCH_CHECK();
-  return {norm, coef};
+  out.fold = DdlNormFold{out.partials.data_ptr<double>(), blocks, mul,
+                         max_norm, out.norm.data_ptr<float>(),
+                         out.coef.data_ptr<float>()};
+  return out;
 }
 
-// The gradients that these plans collected, as one vector.
-std::tuple<at::Tensor, at::Tensor> adamw_grad_norm(
-    const std::vector<std::shared_ptr<AdamWPlan>>& plans, double grad_mul,
-    double max_norm) {
-  TORCH_CHECK(!plans.empty(), "no plans");
-  std::vector<NormList> lists;
-  for (const auto& p : plans) {
-    TORCH_CHECK(p->device() == plans[0]->device(),
-                "clipping needs all parameters on one device");
-    lists.push_back(NormList{p->grad_rows(), p->dtype()});
+// (lr, beta1, beta2, eps, weight_decay, seed) of a plan's group
+using Hyper = std::tuple<double, double, double, double, double, int64_t>;
+
+// One step of all plans, which have collected their gradients.  max_norm 0:
+// no clipping; otherwise returns the gradients' norm.
+c10::optional<at::Tensor> adamw_step(
+    const std::vector<std::shared_ptr<AdamWPlan>>& plans,
+    const std::vector<Hyper>& hyper, double grad_mul, double max_norm) {
+  TORCH_CHECK(plans.size() == hyper.size(), "numbers for each plan");
+  Norm norm;
+  const bool clip = max_norm != 0 && !plans.empty();
+  if (clip) {
+    std::vector<NormList> lists;
+    for (const auto& p : plans) {
+      TORCH_CHECK(p->device() == plans[0]->device(),
+                  "clipping needs all parameters on one device");
+      lists.push_back(NormList{p->grad_rows(), p->dtype()});
+    }
+    c10::DeviceGuard guard(plans[0]->device());
+    norm = norm_of(lists, plans[0]->device(), grad_mul, max_norm);
   }
-  c10::DeviceGuard guard(plans[0]->device());
-  return norm_of(lists, plans[0]->device(), grad_mul, max_norm);
+  for (size_t i = 0; i < plans.size(); ++i) {
+    const auto& [lr, beta1, beta2, eps, decay, seed] = hyper[i];
+    plans[i]->step(DdlAdamScalars{lr, beta1, beta2, eps, decay,
+                                  (float)grad_mul, (uint32_t)seed},
+                   clip && i == 0 ? &norm.fold : nullptr,
+                   clip ? norm.fold.coef : nullptr);
+  }
+  if (!clip) return c10::nullopt;
+  return norm.norm;
 }
 
-at::Tensor clip_grads(const std::vector<at::Tensor>& grads, double grad_mul,
+// The gradients of these parameters.
+at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
                       double max_norm) {
-  TORCH_CHECK(!grads.empty(), "no gradients");
-  const auto device = grads[0].device();
   std::vector<NormList> lists(3);
   for (int i = 0; i < 3; ++i) lists[i].dtype = i;
   std::unordered_set<const void*> seen;
-  for (const auto& g : grads) {
+  seen.reserve(2 * params.size());
+  c10::optional<c10::Device> device;
+  for (const auto& p : params) {
+    const at::Tensor& g = p.grad();
+    if (!g.defined()) continue;
     check_grad(g);
-    TORCH_CHECK(g.is_cuda() && g.device() == device,
+    if (!device.has_value()) device = g.device();
+    TORCH_CHECK(g.is_cuda() && g.device() == *device,
                 "all gradients are on one GPU");
     TORCH_CHECK(dense(g), "a gradient is not dense in memory");
     const int dtype = code_of(g.scalar_type());
@@ -282,13 +313,15 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& grads, double grad_mul,
                 "a gradient appears twice");
     lists[dtype].rows.push_back(DdlGradTensor{g.data_ptr(), g.numel()});
   }
-  c10::DeviceGuard guard(device);
-  auto [norm, coef] = norm_of(lists, device, grad_mul, max_norm);
+  TORCH_CHECK(device.has_value(), "no gradients");
+  c10::DeviceGuard guard(*device);
+  Norm norm = norm_of(lists, *device, grad_mul, max_norm);
+  ddl_grad_norm_fold(&norm.fold, stream_now());
   for (const auto& l : lists)
     ddl_grad_scale(l.rows.data(), (int64_t)l.rows.size(), l.dtype,
-                   coef.const_data_ptr<float>(), stream_now());
+                   norm.fold.coef, stream_now());
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  return norm;
+  return norm.norm;
 }
 
 }  // namespace
@@ -299,9 +332,7 @@ void bind_adamw(pybind11::module& m) {
                           AdamWPlan::Maybe, AdamWPlan::Maybe, AdamWPlan::Maybe,
                           AdamWPlan::Maybe, AdamWPlan::Maybe,
                           std::vector<int64_t>, int64_t>())
-      .def("need", &AdamWPlan::need)
-      .def("collect", &AdamWPlan::collect)
-      .def("step", &AdamWPlan::step);
-  m.def("adamw_grad_norm", &adamw_grad_norm);
+      .def("collect", &AdamWPlan::collect);
+  m.def("adamw_step", &adamw_step);
   m.def("clip_grads", &clip_grads);
 }

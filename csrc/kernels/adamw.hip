@@ -29,6 +29,8 @@
 #include "common.h"
 #include "train_api.h"
 
+#include <cmath>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -112,15 +114,53 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x;
 }
 
-__global__ void prepare_k(PrepArgs a, double lr, double beta1, double beta2,
-                          uint32_t seed, Scalars* out) {
+// Sum of up to 1024 threads, in the same order every time, to all of them.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[16];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off, WAVE);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double total = 0.0;
+  for (int i = 0; i < (int)blockDim.x / WAVE; ++i) total += part[i];
+  return total;
+}
+
+// norm = sqrt(sum of the partial sums) * mul; the coefficient that brings it
+// to max_norm.  NaN stays NaN, as in torch's clip_grad_norm_.
+__device__ __forceinline__ void fold_norm(const DdlNormFold& f) {
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < f.blocks; i += blockDim.x)
+    sum += f.partials[i];
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) {
+    const float n = (float)(sqrt(sum) * f.mul);
+    *f.norm = n;
+    const float k = (float)f.max_norm / (n + 1e-6f);
+    *f.coef = k >= 1.f ? 1.f : k;
+  }
+}
+
+constexpr int FOLD_THREADS = 1024;
+
+__global__ __launch_bounds__(FOLD_THREADS) void fold_norm_k(DdlNormFold f) {
+  fold_norm(f);
+}
+
+// One thread a tensor; the fold of the norm rides along.  beta^t is
+// exp(t log beta) in 64 bits, good to 2^-45 for the steps that matter.
+__global__ __launch_bounds__(FOLD_THREADS) void prepare_k(
+    PrepArgs a, double lr, double log_beta1, double log_beta2, uint32_t seed,
+    Scalars* out, DdlNormFold f) {
+  if (f.partials) fold_norm(f);
   const int i = threadIdx.x;
   if (i >= a.count) return;
   const float t = *a.step[i] + 1.f;
   *a.step[i] = t;
   Scalars s;
-  s.step_size = (float)(lr / (1.0 - pow(beta1, (double)t)));
-  s.inv_sqrt_c2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
+  s.step_size = (float)(lr / -expm1((double)t * log_beta1));
+  s.inv_sqrt_c2 = (float)(1.0 / sqrt(-expm1((double)t * log_beta2)));
   const uint32_t stream = mix(seed + 0x9E3779B9u * (a.index[i] + 1u));
   s.key = mix(stream + (uint32_t)t);
   s.pad = 0;
@@ -339,17 +379,6 @@ __global__ __launch_bounds__(THREADS) void adamw8_k(
 
 // ---- gradient norm and scaling --------------------------------------------
 
-__device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[16];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off, WAVE);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < (int)blockDim.x / WAVE; ++i) total += part[i];
-  return total;
-}
-
 // Squares are summed in 64 bits: a float32 gradient of 2e19 has a square
 // that 32 bits do not hold, and the sum's order does not matter to 32 bits.
 template <typename T>
@@ -361,16 +390,24 @@ __global__ __launch_bounds__(THREADS) void grad_norm_k(NormArgs a,
   const int64_t end = min(a.n[ti], begin + a.chunk);
   const bool aligned = ((uintptr_t)g & 15) == 0;
   double sum = 0.0;
-  if (aligned) {
-    for (int64_t i = begin + threadIdx.x * 8; i + 8 <= end;
-         i += THREADS * 8) {
-      const Vec8<T> x = load8(g + i);
+  auto add = [&](const Vec8<T>& x) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const double d = (double)to_f32(x.v[j]);
-        sum += d * d;
-      }
+    for (int j = 0; j < 8; ++j) {
+      const double d = (double)to_f32(x.v[j]);
+      sum += d * d;
     }
+  };
+  if (aligned) {
+    constexpr int TURN = THREADS * 8;
+    int64_t i = begin + threadIdx.x * 8;
+    for (; i + 3 * TURN + 8 <= end; i += 4 * TURN) {
+      Vec8<T> x[4];  // four loads under way
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = load8(g + i + q * TURN);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) add(x[q]);
+    }
+    for (; i + 8 <= end; i += TURN) add(load8(g + i));
   }
   const int64_t done = aligned ? begin + ((end - begin) & ~7) : begin;
   for (int64_t i = done + threadIdx.x; i < end; i += THREADS) {
@@ -379,24 +416,6 @@ __global__ __launch_bounds__(THREADS) void grad_norm_k(NormArgs a,
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
-}
-
-__global__ __launch_bounds__(1024) void grad_norm_finish_k(
-    const double* partials, int64_t blocks, double mul, double max_norm,
-    float* norm, float* coef) {
-  double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < blocks; i += blockDim.x)
-    sum += partials[i];
-  sum = block_sum(sum);
-  if (threadIdx.x == 0) {
-    const float n = (float)(sqrt(sum) * mul);
-    *norm = n;
-    if (coef) {
-      // NaN stays NaN, as in torch's clip_grad_norm_
-      const float k = (float)max_norm / (n + 1e-6f);
-      *coef = k >= 1.f ? 1.f : k;
-    }
-  }
 }
 
 template <typename T>
@@ -425,19 +444,33 @@ __global__ __launch_bounds__(THREADS) void grad_scale_k(
 
 // ---- host ------------------------------------------------------------------
 
-constexpr int CHUNK = 8192;
 constexpr int64_t MAX_BLOCKS = 1 << 23;  // a grid holds below 2^32 threads
-static_assert(CHUNK % MOMENT_BLOCK == 0, "a chunk holds whole blocks");
+
+// Elements a block takes.  8192 of them (four turns of its threads) hide the
+// block's beginning: ResNet-50's step takes 148 us, with 2048 155.  Few
+// elements are spread over more blocks: 2 million in 2048s take 10.9 us, in
+// 8192s 12.4.
+int chunk_of(int64_t total) {
+  constexpr int TURN = THREADS * 8;
+  static_assert(TURN % MOMENT_BLOCK == 0, "a chunk holds whole blocks");
+  return total >= ((int64_t)1 << 23) ? 4 * TURN : TURN;
+}
+
+template <typename Row> int64_t total_of(const Row* t, int64_t count) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += t[i].n;
+  return total;
+}
 
 bool takes16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Hands `launch` the tensors in groups of at most MAX, with the blocks that
 // each group needs and the place of its first tensor.
 template <typename A, int MAX, typename Size, typename Fill, typename Launch>
-void in_groups(int64_t count, Size size, Fill fill, Launch launch) {
+void in_groups(int64_t count, int chunk, Size size, Fill fill, Launch launch) {
   A a;
   a.count = 0;
-  a.chunk = CHUNK;
+  a.chunk = chunk;
   int64_t blocks = 0, start = 0;
   auto flush = [&](int64_t next) {
     if (blocks) launch(a, (int)blocks, start);
@@ -446,7 +479,7 @@ void in_groups(int64_t count, Size size, Fill fill, Launch launch) {
     start = next;
   };
   for (int64_t i = 0; i < count; ++i) {
-    const int64_t more = cdiv(size(i), CHUNK);
+    const int64_t more = cdiv(size(i), chunk);
     if (a.count == MAX || blocks + more > MAX_BLOCKS) flush(i);
     fill(a, a.count, i);
     a.first[a.count++] = (int)blocks;
@@ -466,6 +499,7 @@ template <typename T, bool MASTER>
 void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
                int bits, const Scalars* ws, const float* coef,
                hipStream_t s) {
+  const int chunk = chunk_of(total_of(t, count));
   auto size = [&](int64_t i) { return t[i].n; };
   auto common = [&](T32& r, int64_t i) {
     r.p = t[i].p;
@@ -478,7 +512,7 @@ void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
   };
   if (bits == 32) {
     using A = Args<T32, MAX_T32>;
-    in_groups<A, MAX_T32>(count, size,
+    in_groups<A, MAX_T32>(count, chunk, size,
         [&](A& a, int k, int64_t i) {
           a.aligned[k] = common(a.t[k], i) && takes16(t[i].m) &&
                          takes16(t[i].v);
@@ -488,7 +522,7 @@ void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
         });
   } else {
     using A = Args<T8, MAX_T8>;
-    in_groups<A, MAX_T8>(count, size,
+    in_groups<A, MAX_T8>(count, chunk, size,
         [&](A& a, int k, int64_t i) {
           a.aligned[k] = common(a.t[k], i) &&
                          ((uintptr_t)t[i].m & 7) == 0 &&
@@ -504,7 +538,7 @@ void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
 
 template <typename Launch>
 void norm_groups(const DdlGradTensor* t, int64_t count, Launch launch) {
-  in_groups<NormArgs, MAX_NORM>(count,
+  in_groups<NormArgs, MAX_NORM>(count, chunk_of(total_of(t, count)),
       [&](int64_t i) { return t[i].n; },
       [&](NormArgs& a, int k, int64_t i) {
         a.g[k] = t[i].g;
@@ -522,7 +556,10 @@ int64_t ddl_adamw_ws_bytes(int64_t count) {
 }
 
 void ddl_adamw_prepare(const DdlAdamTensor* t, int64_t count,
-                       const DdlAdamScalars* c, void* ws, hipStream_t s) {
+                       const DdlAdamScalars* c, void* ws,
+                       const DdlNormFold* fold, hipStream_t s) {
+  DdlNormFold f{};
+  if (fold) f = *fold;
   for (int64_t at = 0; at < count; at += MAX_PREP) {
     PrepArgs a;
     a.count = (int)std::min<int64_t>(MAX_PREP, count - at);
@@ -530,8 +567,11 @@ void ddl_adamw_prepare(const DdlAdamTensor* t, int64_t count,
       a.step[k] = t[at + k].step;
       a.index[k] = t[at + k].index;
     }
-    prepare_k<<<1, MAX_PREP, 0, s>>>(a, c->lr, c->beta1, c->beta2, c->seed,
-                                     (Scalars*)ws + at);
+    const int threads = f.partials ? FOLD_THREADS : MAX_PREP;
+    prepare_k<<<1, threads, 0, s>>>(a, c->lr, std::log(c->beta1),
+                                    std::log(c->beta2), c->seed,
+                                    (Scalars*)ws + at, f);
+    f = DdlNormFold{};
   }
 }
 
@@ -548,8 +588,9 @@ void ddl_adamw(const DdlAdamTensor* t, int64_t count,
 }
 
 int64_t ddl_grad_norm_blocks(const DdlGradTensor* t, int64_t count) {
+  const int chunk = chunk_of(total_of(t, count));
   int64_t blocks = 0;
-  for (int64_t i = 0; i < count; ++i) blocks += cdiv(t[i].n, CHUNK);
+  for (int64_t i = 0; i < count; ++i) blocks += cdiv(t[i].n, chunk);
   return blocks;
 }
 
@@ -565,11 +606,8 @@ void ddl_grad_norm_partials(const DdlGradTensor* t, int64_t count, int dtype,
   });
 }
 
-void ddl_grad_norm_finish(const double* partials, int64_t blocks, double mul,
-                          double max_norm, float* norm, float* coef,
-                          hipStream_t s) {
-  grad_norm_finish_k<<<1, 1024, 0, s>>>(partials, blocks, mul, max_norm, norm,
-                                        coef);
+void ddl_grad_norm_fold(const DdlNormFold* f, hipStream_t s) {
+  fold_norm_k<<<1, FOLD_THREADS, 0, s>>>(*f);
 }
 
 void ddl_grad_scale(const DdlGradTensor* t, int64_t count, int dtype,

@@ -36,26 +36,35 @@ struct DdlGradTensor {
 
 #define DDL_MOMENT_BLOCK 256
 
-// Step counts += 1, and the numbers that follow from them for each tensor.
+// Partial sums of squares -> norm = sqrt(sum) * mul and
+// coef = min(1, max_norm / (norm + 1e-6)).
+struct DdlNormFold {
+  const double* partials;
+  int64_t blocks;
+  double mul, max_norm;
+  float* norm;
+  float* coef;
+};
+
+// Step counts += 1, and the numbers that follow from them for each tensor;
+// the fold, where there is one, in the same launch.
 // ws: ddl_adamw_ws_bytes(count) bytes.
 int64_t ddl_adamw_ws_bytes(int64_t count);
 void ddl_adamw_prepare(const DdlAdamTensor* t, int64_t count,
-                       const DdlAdamScalars* c, void* ws, hipStream_t s);
+                       const DdlAdamScalars* c, void* ws,
+                       const DdlNormFold* fold, hipStream_t s);
 // The update of all tensors.  coef: device scalar that multiplies every
 // gradient (clipping), or null.
 void ddl_adamw(const DdlAdamTensor* t, int64_t count,
                const DdlAdamScalars* c, int dtype, int bits, const void* ws,
                const float* coef, hipStream_t s);
 
-// Global gradient norm.  partials: ddl_grad_norm_blocks() doubles for each
-// list, one after the other; ddl_grad_norm_finish folds `blocks` of them:
-// norm = sqrt(sum) * mul, coef = min(1, max_norm / (norm + 1e-6)).
+// Global gradient norm: partial sums of one list, ddl_grad_norm_blocks()
+// doubles, to be folded together with those of other lists.
 int64_t ddl_grad_norm_blocks(const DdlGradTensor* t, int64_t count);
 void ddl_grad_norm_partials(const DdlGradTensor* t, int64_t count, int dtype,
                             double* partials, hipStream_t s);
-void ddl_grad_norm_finish(const double* partials, int64_t blocks, double mul,
-                          double max_norm, float* norm, float* coef,
-                          hipStream_t s);
+void ddl_grad_norm_fold(const DdlNormFold* f, hipStream_t s);
 // g *= *coef; nothing is read or written where *coef is 1.
 void ddl_grad_scale(const DdlGradTensor* t, int64_t count, int dtype,
                     const float* coef, hipStream_t s);

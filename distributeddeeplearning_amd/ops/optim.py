@@ -459,9 +459,8 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params = [p for g in self.param_groups for p in g["params"]]
-        if any(p.is_cuda for p in params):
-            self._step_gpu(params)
+        if any(p.is_cuda for g in self.param_groups for p in g["params"]):
+            self._step_gpu()
         else:
             self._step_cpu()
         return loss
@@ -489,30 +488,25 @@ class FusedAdamW(torch.optim.Optimizer):
                                      group["state_bits"])
                 self._plans.append((plan, group, [p for _, p in members]))
 
-    def _step_gpu(self, params):
+    def _step_gpu(self):
         if self._plans is None:
             self._build_plans()
         missing = False
         for plan, group, members in self._plans:
-            for i in plan.need():  # the first gradient of a parameter
+            for i in plan.collect():  # the first gradient of a parameter
                 self._init_state(members[i], group["state_bits"])
                 missing = True
         if missing:
             self._build_plans()
-        for plan, _, _ in self._plans:
-            plan.collect()
-        grad_mul = 1.0 / self.grad_scale
-        coef = None
-        if self.max_grad_norm is not None and self._plans:
-            ext = load_kernels_ext()
-            self.grad_norm, coef = ext.adamw_grad_norm(
-                [plan for plan, _, _ in self._plans], grad_mul,
-                float(self.max_grad_norm))
-        for plan, group, _ in self._plans:
-            beta1, beta2 = group["betas"]
-            plan.step(float(group["lr"]), float(beta1), float(beta2),
-                      float(group["eps"]), float(group["weight_decay"]),
-                      grad_mul, int(group["seed"]) & 0xFFFFFFFF, coef)
+            for plan, _, _ in self._plans:
+                plan.collect()
+        norm = load_kernels_ext().adamw_step(
+            [plan for plan, _, _ in self._plans],
+            [(g["lr"], *g["betas"], g["eps"], g["weight_decay"],
+              int(g["seed"]) & 0xFFFFFFFF) for _, g, _ in self._plans],
+            1.0 / self.grad_scale, self.max_grad_norm or 0.0)
+        if norm is not None:
+            self.grad_norm = norm
 
     def _step_cpu(self):
         mul = 1.0 / self.grad_scale
@@ -596,21 +590,22 @@ def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
     not caught: it makes the gradients zero or NaN.
 
     Under data parallelism call it after ``DistributedOptimizer.synchronize``;
-    every rank then computes the same norm.  Two launches read and fold, a
-    third scales; gradients are not touched where the norm is within bounds.
+    every rank then computes the same norm.  Gradients are not touched where
+    the norm is within bounds.
     """
     params = [params] if torch.is_tensor(params) else list(params)
     if not max_norm > 0:
         raise ValueError(f"max_norm must be positive: {max_norm}")
     if not grad_scale > 0:
         raise ValueError(f"grad_scale must be positive: {grad_scale}")
-    grads = [p.grad for p in params if p.grad is not None]
-    if not grads:
+    first = next((p.grad for p in params if p.grad is not None), None)
+    if first is None:
         device = params[0].device if params else None
         return torch.zeros((), dtype=torch.float32, device=device)
-    if grads[0].is_cuda:
-        return load_kernels_ext().clip_grads(grads, 1.0 / grad_scale,
+    if first.is_cuda:
+        return load_kernels_ext().clip_grads(params, 1.0 / grad_scale,
                                              float(max_norm))
+    grads = [p.grad for p in params if p.grad is not None]
     norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
     if not float(coef) == 1.0:
         for g in grads:
