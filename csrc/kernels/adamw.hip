@@ -400,12 +400,10 @@ __global__ __launch_bounds__(THREADS) void grad_norm_k(NormArgs a,
   if (aligned) {
     constexpr int TURN = THREADS * 8;
     int64_t i = begin + threadIdx.x * 8;
-    for (; i + 3 * TURN + 8 <= end; i += 4 * TURN) {
-      Vec8<T> x[4];  // four loads under way
-#pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] = load8(g + i + q * TURN);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) add(x[q]);
+    for (; i + TURN + 8 <= end; i += 2 * TURN) {
+      const Vec8<T> x = load8(g + i), y = load8(g + i + TURN);
+      add(x);
+      add(y);
     }
     for (; i + 8 <= end; i += TURN) add(load8(g + i));
   }
@@ -446,14 +444,13 @@ __global__ __launch_bounds__(THREADS) void grad_scale_k(
 
 constexpr int64_t MAX_BLOCKS = 1 << 23;  // a grid holds below 2^32 threads
 
-// Elements a block takes.  8192 of them (four turns of its threads) hide the
-// block's beginning: ResNet-50's step takes 148 us, with 2048 155.  Few
-// elements are spread over more blocks: 2 million in 2048s take 10.9 us, in
-// 8192s 12.4.
+// Elements a block takes: two turns of its threads.  ResNet-50's step takes
+// 141 us so, 146 with four turns; few elements are spread over more blocks:
+// 2 million take 10.4 us in single turns, 12.4 in four.
 int chunk_of(int64_t total) {
   constexpr int TURN = THREADS * 8;
   static_assert(TURN % MOMENT_BLOCK == 0, "a chunk holds whole blocks");
-  return total >= ((int64_t)1 << 23) ? 4 * TURN : TURN;
+  return total >= ((int64_t)1 << 23) ? 2 * TURN : TURN;
 }
 
 template <typename Row> int64_t total_of(const Row* t, int64_t count) {
