@@ -59,19 +59,19 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
   for (int i = 0; i < MT; ++i)
     xrow[i] = x + min((int64_t)i * 16 + c, e.m - 1) * ldx;
 
-  f32x4 acc[MT] = {};
+  f32x4 acc[MT][1] = {};
   using F = typename Frag<T>::type;
   auto take = [&](int64_t chunk, auto lines, auto whole) {
     constexpr int N = decltype(lines)::value;
     constexpr bool WHOLE = decltype(whole)::value;
-    F wf[N][2], xf[N][2][MT];
+    F wf[N][2][1], xf[N][2][MT];
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t k =
             (chunk + u * WAVES) * CHUNK + h * (CHUNK / 2) + g * E;
-        wf[u][h] = piece<T, WHOLE>(wrow, k, r);
+        wf[u][h][0] = piece<T, WHOLE>(wrow, k, r);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           xf[u][h][i] = piece<T, WHOLE>(xrow[i], k, r);
@@ -79,10 +79,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          acc[i] = mma(wf[u][h], xf[u][h][i], acc[i]);
+      for (int h = 0; h < 2; ++h) multiply(acc, xf[u][h], wf[u][h]);
   };
   const int64_t whole = r / CHUNK;
   int64_t k0 = wave;
@@ -96,7 +93,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sums[wave][i][c][g * 4 + q] = acc[i][q];
+    for (int q = 0; q < 4; ++q) sums[wave][i][c][g * 4 + q] = acc[i][0][q];
   __syncthreads();
   const int t = threadIdx.x;
   if (t < MT * 32) {
@@ -128,7 +125,7 @@ void run_few(const DdlProduct* p, hipStream_t s) {
 
 // ---- backward of the activation, bias gradient ------------------------------
 
-constexpr int BWD_ROWS = 32;   // rows a block sums
+constexpr int BWD_ROWS = 16;   // rows a block sums
 constexpr int BWD_COLS = 256;  // 32 threads of 8 columns
 
 // Elements j..j+7 of a row of n, zeros behind its end; it may begin anywhere.
@@ -199,7 +196,8 @@ __global__ __launch_bounds__(256) void act_bwd_k(
 
 template <typename T>
 __global__ __launch_bounds__(256) void fold_bias_k(DdlBiasFold f) {
-  fold_bias<T>(f, global_tid());
+  __shared__ __align__(16) char smem[256 * sizeof(double)];
+  fold_bias<T>(f, blockIdx.x, smem);
 }
 
 // ---- rows that do not begin or end at 16 bytes -------------------------------
@@ -302,7 +300,7 @@ void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
 }
 
 void ddl_fold_bias(const DdlBiasFold* f, int dtype, hipStream_t s) {
-  const unsigned blocks = (unsigned)cdiv(f->n, 256);
+  const unsigned blocks = (unsigned)cdiv(f->n, FOLD_COLS);
   switch (dtype) {
     case 0: fold_bias_k<float><<<blocks, 256, 0, s>>>(*f); break;
     case 1: fold_bias_k<bf16><<<blocks, 256, 0, s>>>(*f); break;

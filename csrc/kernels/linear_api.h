@@ -44,7 +44,7 @@ int ddl_few_rows(void);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
 // dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of
-// 8), and the column sums of dz before its rounding, of 32 rows each: partials
+// 8), and the column sums of dz before its rounding, of 16 rows each: partials
 // holds ddl_bias_chunks(m) * n floats.  z is float32 (z_f32), or for act 1 the
 // output in the tensors' dtype.  dz or partials may be null.
 int64_t ddl_bias_chunks(int64_t m);

@@ -120,11 +120,33 @@ __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
+// Of the four instructions that a float32 fragment pair takes, number e.
+__device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// acc[i][j] += b[j] a[i].  For float32 the four instructions of a pair depend
+// on one another: they are spread over the pairs.
+template <int MI, int NI>
+__device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI],
+                                         const f32x4 (&a)[MI],
+                                         const f32x4 (&b)[NI]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-  return c;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        acc[i][j] = mma(b[j][e], a[i][e], acc[i][j]);
+}
+
+template <typename F, int MI, int NI>
+__device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI],
+                                         const F (&a)[MI], const F (&b)[NI]) {
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = mma(b[j], a[i], acc[i][j]);
 }
 
 // ---- epilogue --------------------------------------------------------------
@@ -474,12 +496,6 @@ __device__ __forceinline__ void product_block(const Product& p, unsigned id,
 #pragma unroll
     for (int f = 0; f < MI; ++f) af[f] = ta.read(la, lane, wm, f, kk);
   };
-  auto multiply = [&](const F (&af)[MI], const F (&bf)[NI]) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = mma(bf[j], af[i], acc[i][j]);
-  };
   constexpr int PER = sizeof(T) == 4 ? 4 : 1;  // instructions a fragment pair
   constexpr int READS = MI * TA::READS + NI * TB::READS;
   constexpr int LOADS = TA::LOADS + TB::LOADS;
@@ -492,18 +508,18 @@ __device__ __forceinline__ void product_block(const Product& p, unsigned id,
     for (int64_t t = t0; t + 1 < t1; ++t) {
       const int next = stage + 1 < STAGES ? stage + 1 : 0;
       read(a1, b1, stage, 1);
-      multiply(a0, b0);
+      multiply(acc, a0, b0);
       interleave<READS, MI * NI * PER, 0>();
       meet<(STAGES - 2) * LOADS>();
       load(t + STAGES, stage);
       read(a0, b0, next, 0);
-      multiply(a1, b1);
+      multiply(acc, a1, b1);
       interleave<READS, MI * NI * PER, LOADS>();
       stage = next;
     }
     read(a1, b1, stage, 1);
-    multiply(a0, b0);
-    multiply(a1, b1);
+    multiply(acc, a0, b0);
+    multiply(acc, a1, b1);
   }
 
   meet<0>();
@@ -519,15 +535,27 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
       p, xcd_swizzle(blockIdx.x, gridDim.x), smem);
 }
 
-// Column j of the bias gradient: the fold of act_bwd_k's partial sums.
+// The fold of act_bwd_k's partial sums: FOLD_COLS columns a block of 256.
+constexpr int FOLD_COLS = 32;
+
 template <typename T>
-__device__ __forceinline__ void fold_bias(const DdlBiasFold& f,
-                                          int64_t j) {
-  if (j >= f.n) return;
-  double sum = 0.0;  // as many chunks as there are rows / 32
-#pragma unroll 8
-  for (int64_t c = 0; c < f.chunks; ++c) sum += f.partials[c * f.n + j];
-  ((T*)f.dbias)[j] = from_f32<T>((float)sum);
+__device__ __forceinline__ void fold_bias(const DdlBiasFold& f, int64_t block,
+                                          char* smem) {
+  constexpr int LANES = 256 / FOLD_COLS;
+  double* part = reinterpret_cast<double*>(smem);
+  const int col = threadIdx.x % FOLD_COLS, lane = threadIdx.x / FOLD_COLS;
+  const int64_t j = block * FOLD_COLS + col;
+  double sum = 0.0;  // as many chunks as there are rows / 16
+  if (j < f.n)
+#pragma unroll 4
+    for (int64_t c = lane; c < f.chunks; c += LANES)
+      sum += f.partials[c * f.n + j];
+  part[threadIdx.x] = sum;
+  __syncthreads();
+  if (lane == 0 && j < f.n) {
+    for (int k = 1; k < LANES; ++k) sum += part[k * FOLD_COLS + col];
+    ((T*)f.dbias)[j] = from_f32<T>((float)sum);
+  }
 }
 
 // Both products of a small layer's backward pass and the fold of its bias
@@ -544,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void backward_small_k(
   } else if (id < nx + nw) {
     product_block<T, 64, 64, 4, 1, 4, true, true>(dw, id - nx, smem);
   } else {
-    fold_bias<T>(bias, (int64_t)(id - nx - nw) * 256 + threadIdx.x);
+    fold_bias<T>(bias, id - nx - nw, smem);
   }
 }
 
@@ -752,7 +780,8 @@ void run_backward_small(DdlProduct dx, DdlProduct dw, const DdlBiasFold& bias,
   }
   const Product x = product_of<T>(&dx), w = product_of<T>(&dw);
   const int64_t blocks = (int64_t)x.tiles_m * x.tiles_n +
-                         (int64_t)w.tiles_m * w.tiles_n + cdiv(bias.n, 256);
+                         (int64_t)w.tiles_m * w.tiles_n +
+                         cdiv(bias.n, FOLD_COLS);
   backward_small_k<T><<<(unsigned)blocks, 256, 0, s>>>(x, w, bias);
 }
 
