@@ -43,6 +43,14 @@ class TrainConfig:
     lars_eta: float = 0.001
     loss_scale: float = 0.0          # 0 = dynamic (fp16 only)
     zero_init_residual: bool = False
+    optimizer: str = "sgd"           # sgd (momentum, LARS) | adamw
+    adam_beta1: float = 0.9
+    adam_beta2: float = 0.999
+    adam_eps: float = 1e-8
+    adam_state_bits: int = 32        # 32 | 8 (block-scaled 8-bit moments)
+    clip_norm: float = 0.0           # global gradient norm; 0 = no clipping
+    # VGG: ReLU of the classifier's dense layers in their product's epilogue
+    fused_classifier: bool = False
 
     # comm
     comm: str = "auto"               # auto | native | torchdist | single

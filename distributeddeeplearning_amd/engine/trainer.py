@@ -12,7 +12,7 @@ import torch
 from .. import models as model_zoo
 from ..config import TrainConfig
 from ..data.synthetic import synthetic_loader
-from ..ops import FusedSGD, cast_model_
+from ..ops import FusedAdamW, FusedSGD, cast_model_, clip_grad_norm_
 from ..ops import functional as DF
 from ..parallel import DistributedOptimizer, api
 from . import checkpoint as ckpt
@@ -39,7 +39,8 @@ class Trainer:
             cfg.model, num_classes=cfg.num_classes,
             zero_init_residual=cfg.zero_init_residual,
         ) if cfg.model.startswith("resnet") else model_zoo.build_model(
-            cfg.model, num_classes=cfg.num_classes)
+            cfg.model, num_classes=cfg.num_classes,
+            fused_classifier=cfg.fused_classifier)
         model = model.to(self.device)
         cast_model_(model, dtype, channels_last=cfg.channels_last)
         self.model = model
@@ -58,11 +59,26 @@ class Trainer:
         if cfg.loss_scale > 0:
             self.scaler.growth_interval = 10 ** 9  # static scale
 
-        inner = FusedSGD(
-            model.parameters(), lr=cfg.base_lr, momentum=cfg.momentum,
-            weight_decay=cfg.weight_decay, lars=cfg.lars,
-            lars_eta=cfg.lars_eta, grad_scale=self.scaler.scale,
-        )
+        if cfg.optimizer == "adamw":
+            if cfg.lars:
+                raise ValueError("lars belongs to the sgd optimizer")
+            # clipping rides along in the update
+            inner = FusedAdamW(
+                model.parameters(), lr=cfg.base_lr,
+                betas=(cfg.adam_beta1, cfg.adam_beta2), eps=cfg.adam_eps,
+                weight_decay=cfg.weight_decay, state_bits=cfg.adam_state_bits,
+                max_grad_norm=cfg.clip_norm or None,
+                grad_scale=self.scaler.scale, seed=cfg.seed,
+            )
+        elif cfg.optimizer == "sgd":
+            inner = FusedSGD(
+                model.parameters(), lr=cfg.base_lr, momentum=cfg.momentum,
+                weight_decay=cfg.weight_decay, lars=cfg.lars,
+                lars_eta=cfg.lars_eta, grad_scale=self.scaler.scale,
+            )
+        else:
+            raise ValueError(f"unknown optimizer {cfg.optimizer!r}; "
+                             "available: adamw, sgd")
         self.opt = DistributedOptimizer(
             inner, named_parameters=model.named_parameters(),
             backward_passes_per_step=cfg.backward_passes_per_step,
@@ -170,11 +186,13 @@ class Trainer:
             flats = [b.flat for b in self.opt.buckets.buckets]
             self.opt.optimizer.grad_scale = self.scaler.scale
             if self.scaler.check_and_update(flats):
+                self._clip()
                 self.opt.step()
             # on overflow: skip the update; synchronize() already re-armed
             # the accumulation counters and zero_grad below discards the
             # non-finite gradients, so the next window starts clean
         else:
+            self._clip()
             self.opt.step()
         self.opt.zero_grad()
         if self.bucket_tuner is not None and not self.bucket_tuner.done:
@@ -186,6 +204,15 @@ class Trainer:
                 tl.save()
         self.global_step += 1
         return loss
+
+    def _clip(self) -> None:
+        """Clip the reduced gradients where the optimizer does not by itself."""
+        if not self.cfg.clip_norm or self.cfg.optimizer == "adamw":
+            return
+        if not self.scaler.enabled:  # otherwise they are reduced already
+            self.opt.synchronize()
+        clip_grad_norm_(self.model.parameters(), self.cfg.clip_norm,
+                        grad_scale=self.opt.optimizer.grad_scale)
 
     def train_epoch(self, steps: Optional[int] = None) -> float:
         self.model.train()

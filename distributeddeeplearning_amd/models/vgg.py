@@ -27,7 +27,8 @@ class _FusedConvReLU(Conv2d):
 
 
 class VGG(nn.Module):
-    def __init__(self, cfg=_VGG16_D, num_classes=1000, dropout=0.5):
+    def __init__(self, cfg=_VGG16_D, num_classes=1000, dropout=0.5,
+                 fused_classifier=False):
         super().__init__()
         layers: list[nn.Module] = []
         in_ch = 3
@@ -42,9 +43,16 @@ class VGG(nn.Module):
         # torchvision applies AdaptiveAvgPool2d(7) between features and
         # classifier; at 224x224 input features already end at 7x7 so it is
         # the identity — kept as flatten only.
+        # fused_classifier: ReLU in the dense layers' epilogue; the Identity
+        # keeps the Sequential indices, and with them the parameter names
+        act = "relu" if fused_classifier else "none"
+
+        def relu():
+            return nn.Identity() if fused_classifier else nn.ReLU(inplace=True)
+
         self.classifier = nn.Sequential(
-            Linear(512 * 7 * 7, 4096), nn.ReLU(inplace=True), Dropout(dropout),
-            Linear(4096, 4096), nn.ReLU(inplace=True), Dropout(dropout),
+            Linear(512 * 7 * 7, 4096, activation=act), relu(), Dropout(dropout),
+            Linear(4096, 4096, activation=act), relu(), Dropout(dropout),
             Linear(4096, num_classes),
         )
         for m in self.modules():

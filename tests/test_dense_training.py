@@ -1,0 +1,301 @@
+"""The dense layer, clipping and AdamW together, as a training step uses them:
+in a small network against the same steps in 64 bits, through the trainer and
+its configuration, and data-parallel over gloo."""
+import dataclasses
+
+import pytest
+import torch
+
+from distributeddeeplearning_amd import ops
+from distributeddeeplearning_amd.config import TrainConfig
+from distributeddeeplearning_amd.engine.trainer import Trainer
+from distributeddeeplearning_amd.models import vgg16
+from tests.dist_helpers import run_distributed
+
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+class Net(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.a = ops.Linear(24, 40, activation="gelu")
+        self.b = ops.Linear(40, 40, activation="silu")
+        self.c = ops.Linear(40, 8)
+
+    def forward(self, x):
+        h = self.a(x)
+        return self.c(self.b(h, residual=h))
+
+
+def reference_forward(p, x):
+    f = torch.nn.functional
+    h = f.gelu(x @ p["a.weight"].t() + p["a.bias"])
+    h = f.silu(h @ p["b.weight"].t() + p["b.bias"]) + h
+    return h @ p["c.weight"].t() + p["c.bias"]
+
+
+def batch(step, device="cpu", dtype=torch.float32):
+    gen = torch.Generator().manual_seed(step)
+    return (torch.randn(30, 24, generator=gen).to(device, dtype),
+            torch.randn(30, 8, generator=gen).to(device, dtype))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_training_steps_against_64_bits(device):
+    """Three steps of forward, backward, clip and AdamW in float32.  eps is
+    1e-2, so that a step is a smooth function of the gradient: an error e of
+    a gradient moves a weight by lr e / eps = 0.1 e at most.  Gradients pass
+    six products of up to 40 terms of size about one: the error is below
+    6 * 42 * 2^-24 times sums below 20, 3e-4; so weights are held to
+    3 steps * 0.1 * 3e-4, and the norm to 1e-4 of itself (it averages over
+    all of them)."""
+    torch.manual_seed(0)
+    net = Net()
+    with torch.no_grad():
+        for p in net.parameters():
+            p.copy_(torch.randn(p.shape) * (0.3 if p.dim() > 1 else 0.1))
+    ref = {k: p.detach().double().requires_grad_(True)
+           for k, p in net.named_parameters()}
+    net = net.to(device)
+    opt = ops.FusedAdamW(net.parameters(), lr=1e-3, eps=1e-2,
+                         weight_decay=0.1, max_grad_norm=0.5)
+    ref_opt = torch.optim.AdamW(ref.values(), lr=1e-3, eps=1e-2,
+                                weight_decay=0.1)
+    for step in range(3):
+        x, y = batch(step, device)
+        opt.zero_grad(set_to_none=True)
+        (net(x) - y).square().mean().backward()
+        opt.step()
+        x, y = batch(step)
+        ref_opt.zero_grad()
+        (reference_forward(ref, x.double()) - y.double()
+         ).square().mean().backward()
+        norm = torch.nn.utils.clip_grad_norm_(ref.values(), 0.5)
+        ref_opt.step()
+        assert abs(float(opt.grad_norm) / float(norm) - 1) < 1e-4
+    for k, p in net.named_parameters():
+        assert (p.detach().cpu().double() - ref[k].detach()
+                ).abs().max() < 1e-4, k
+
+
+@gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_training_step(bits):
+    """Forward, backward, clip and step in one graph, replayed."""
+    def build():
+        torch.manual_seed(1)
+        net = Net().cuda()
+        ops.cast_model_(net, torch.bfloat16)
+        return net, ops.FusedAdamW(net.parameters(), lr=1e-2,
+                                   state_bits=bits, max_grad_norm=1.0)
+
+    def step(net, opt, x, y):
+        for p in net.parameters():
+            p.grad = None
+        loss = (net(x).float() - y.float()).square().mean()
+        loss.backward()
+        opt.step()
+
+    x, y = (t.cuda().bfloat16() for t in batch(0))
+    nets = [build() for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for net, opt in nets:
+            step(net, opt, x, y)
+    torch.cuda.current_stream().wait_stream(side)
+    for net, _ in nets:
+        for p in net.parameters():
+            p.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*nets[0], x, y)
+    for k in range(4):
+        new = batch(k + 1)
+        x.copy_(new[0])
+        y.copy_(new[1])
+        graph.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            step(*nets[1], x, y)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        for p, q in zip(nets[0][0].parameters(), nets[1][0].parameters()):
+            assert torch.equal(p, q)
+
+
+# ---- trainer ---------------------------------------------------------------
+
+def _cfg(**kw):
+    base = dict(model="resnet18", image_size=32, num_classes=10, batch_size=4,
+                dtype="fp32", device="cpu", comm="single", warmup_epochs=0,
+                base_lr=1e-3)
+    base.update(kw)
+    return TrainConfig(**base)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(optimizer="adamw"), dict(optimizer="adamw", adam_state_bits=8,
+                                  clip_norm=1.0),
+    dict(optimizer="sgd", clip_norm=0.5),
+    dict(optimizer="adamw", dtype="fp16", clip_norm=1.0, loss_scale=256.0),
+    dict(optimizer="sgd", dtype="fp16", clip_norm=1.0, loss_scale=256.0),
+])
+@pytest.mark.parametrize("device", DEVICES)
+def test_trainer(kw, device):
+    if device == "cpu" and kw.get("dtype") == "fp16":
+        pytest.skip("float16 convolutions need the GPU")
+    tr = Trainer(_cfg(device=device, **kw), steps_per_epoch=10)
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    it = tr.data_iter()
+    for _ in range(2):
+        loss = tr.train_step(*next(it))
+    assert torch.isfinite(loss)
+    # of the float32 masters: a float16 weight near one does not move by less
+    # than 2^-11, and two steps of rate 1e-3 with a gradient of norm one are
+    # less than that in most weights
+    moved = [not torch.equal(tr.opt.state[p].get("master", p).float(),
+                             q.float())
+             for p, q in zip(tr.model.parameters(), before)]
+    assert all(moved)
+    if kw["optimizer"] == "adamw":
+        st = tr.opt.state[next(tr.model.parameters())]
+        assert float(st["step"]) == 2
+        assert (tr.opt.optimizer.grad_norm is not None) == ("clip_norm" in kw)
+
+
+def test_trainer_clips_sgd_by_the_unscaled_norm():
+    """One step without momentum moves the weights by lr times the clipped
+    gradient, whose norm is the bound."""
+    tr = Trainer(_cfg(clip_norm=0.01, momentum=0.0, weight_decay=0.0,
+                      base_lr=1.0), steps_per_epoch=10)
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    tr.train_step(*next(tr.data_iter()))
+    lr = tr.lr_sched.last_lr
+    moved = sum(float((p.detach() - q).double().square().sum())
+                for p, q in zip(tr.model.parameters(), before)) ** 0.5
+    # each weight (below 2) is rounded to 2^-24 of itself: 11 million of them
+    # add 3400 * 1.2e-7 at most
+    assert abs(moved - 0.01 * lr) < 0.01 * 1e-4 + 3400 * 1.2e-7
+
+
+def test_trainer_refuses():
+    with pytest.raises(ValueError, match="optimizer"):
+        Trainer(_cfg(optimizer="lion"), steps_per_epoch=1)
+    with pytest.raises(ValueError, match="lars"):
+        Trainer(_cfg(optimizer="adamw", lars=True), steps_per_epoch=1)
+
+
+def test_command_line():
+    cfg = TrainConfig.from_args(["--optimizer", "adamw", "--adam-beta2",
+                                 "0.95", "--adam-state-bits", "8",
+                                 "--clip-norm", "1.5", "--fused-classifier",
+                                 "true"])
+    assert (cfg.optimizer, cfg.adam_beta2, cfg.adam_state_bits, cfg.clip_norm,
+            cfg.fused_classifier) == ("adamw", 0.95, 8, 1.5, True)
+    plain = TrainConfig.from_args([])
+    assert plain.optimizer == "sgd" and not plain.fused_classifier
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint_resumes(bits, tmp_path):
+    from distributeddeeplearning_amd.engine import checkpoint as ckpt
+    kw = dict(optimizer="adamw", adam_state_bits=bits, clip_norm=1.0)
+    a = Trainer(_cfg(**kw), steps_per_epoch=10)
+    batches = [next(a.data_iter()) for _ in range(3)]
+    a.train_step(*batches[0])
+    path = str(tmp_path / "c.pt")
+    ckpt.save(path, a.model, a.opt, 0, 1, a.scaler)
+    a.train_step(*batches[1])
+    b = Trainer(_cfg(resume=path, seed=7, **kw), steps_per_epoch=10)
+    b.train_step(*batches[1])
+    for p, q in zip(a.model.parameters(), b.model.parameters()):
+        assert torch.equal(p, q)
+
+
+# ---- VGG classifier --------------------------------------------------------
+
+def test_fused_classifier_keeps_names():
+    names = [list(dict(vgg16(num_classes=4, fused_classifier=f)
+                       .named_parameters())) for f in (False, True)]
+    assert names[0] == names[1]
+
+
+@gpu
+def test_fused_classifier_matches():
+    """The classifier alone, bfloat16: each layer rounds sums of size about
+    one once, so outputs and gradients differ by some bfloat16 roundings
+    (2^-8 each): two layers forward and two backward, 8 * 2^-8 of the size."""
+    torch.manual_seed(0)
+    plain = vgg16(num_classes=16, dropout=0.0).classifier.cuda()
+    fused = vgg16(num_classes=16, dropout=0.0,
+                  fused_classifier=True).classifier.cuda()
+    fused.load_state_dict(plain.state_dict())
+    x = torch.randn(40, 25088, device="cuda").relu().bfloat16()
+    grads = []
+    for net in (plain, fused):
+        ops.cast_model_(net, torch.bfloat16)
+        y = net(x)
+        y.float().square().sum().backward()
+        grads.append([y.detach()] + [p.grad for p in net.parameters()])
+    for a, b in zip(*grads):
+        a, b = a.float(), b.float()
+        assert (a - b).norm() <= 8 * 2 ** -8 * a.norm()
+
+
+# ---- data-parallel ---------------------------------------------------------
+
+def _w_adamw(rank, world, bits):
+    from distributeddeeplearning_amd.parallel import DistributedOptimizer, api
+    api.init("torchdist")
+    torch.manual_seed(rank)
+    net = Net()
+    api.broadcast_parameters(net.state_dict(), root_rank=0)
+    opt = DistributedOptimizer(
+        ops.FusedAdamW(net.parameters(), lr=1e-2, state_bits=bits,
+                       max_grad_norm=0.3, eps=1e-3),
+        named_parameters=net.named_parameters(), bucket_bytes=4096)
+    for step in range(3):
+        x, y = batch(step)
+        part = slice(rank * 15, rank * 15 + 15)
+        opt.zero_grad()
+        (net(x[part]) - y[part]).square().mean().backward()
+        opt.step()
+    if rank == 1:  # lost on one rank, sent again by the other
+        for st in opt.state.values():
+            for t in st.values():
+                t.zero_()
+    api.broadcast_optimizer_state(opt, root_rank=0)
+    state = [st[k].float() for st in opt.state.values() for k in sorted(st)]
+    return ([p.detach().clone() for p in net.parameters()], state,
+            float(opt.optimizer.grad_norm))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_two_ranks_agree(bits):
+    (p0, s0, n0), (p1, s1, n1) = run_distributed(_w_adamw, 2, (bits,))
+    assert n0 == n1
+    assert all(torch.equal(a, b) for a, b in zip(p0, p1))
+    assert len(s0) == len(s1) and all(torch.equal(a, b)
+                                      for a, b in zip(s0, s1))
+    if bits == 32:  # and equal one process with the whole batch
+        torch.manual_seed(0)
+        net = Net()
+        opt = ops.FusedAdamW(net.parameters(), lr=1e-2, max_grad_norm=0.3,
+                             eps=1e-3)
+        for step in range(3):
+            x, y = batch(step)
+            opt.zero_grad(set_to_none=True)
+            (net(x) - y).square().mean().backward()
+            opt.step()
+        # a gradient's rounding (below 1e-6 of size one) moves a weight by
+        # lr / eps = 10 of it in each step
+        for p, q in zip(net.parameters(), p0):
+            assert (p.detach() - q).abs().max() < 3 * 10 * 1e-6
+
+
+def test_config_round_trips():
+    cfg = _cfg(optimizer="adamw", clip_norm=1.0)
+    assert TrainConfig(**dataclasses.asdict(cfg)) == cfg
