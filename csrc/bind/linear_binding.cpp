@@ -120,7 +120,8 @@ at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
     p.ldres = row_stride(res);
   }
   if (m == 0 || n == 0) return y;
-  const bool few = m <= ddl_few_rows() && n < ((int64_t)1 << 26);  // its grid
+  const int64_t floats = ddl_product_plan(&p);
+  const bool few = ddl_few_rows_pay(&p, fits(x) && fits(w));
   if (few) {
     x = inner_contiguous(x);
     w = inner_contiguous(w);
@@ -134,7 +135,7 @@ at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
   if (few)
     ddl_product_few(&p, stream_now());
   else
-    product(p, ddl_product_plan(&p), x);
+    product(p, floats, x);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return y;
 }

@@ -17,12 +17,13 @@ namespace {
 
 // ---- forward for few rows ----------------------------------------------------
 
-// Up to 16 MT rows of x: what counts is one pass over W.  A block takes 16
+// Up to 16 rows of x: what counts is one pass over W.  A block takes 16
 // outputs; its waves take turns along the inputs and read W straight into
-// fragments (16 lines of 64 bytes an instruction, a whole line in two), many
-// loads ahead; their sums meet in LDS, in the waves' order.  No slabs and no
-// second launch.  Rows may begin and end anywhere.
-constexpr int FEW_UNROLL = 4;  // lines of W a lane has under way
+// fragments (16 lines of 64 bytes an instruction, a whole line in two), four
+// lines ahead; their sums meet in LDS, in the waves' order.  No slabs and no
+// second launch.  Rows may begin and end anywhere.  bf16, 1 x 4096 -> 4096:
+// 9.1 us with the launch, where W alone takes 6.6 at 5.07 TB/s.
+constexpr int FEW_UNROLL = 4;
 
 // 16 bytes of a row; WHOLE: they end before r.
 template <typename T, bool WHOLE>
@@ -41,30 +42,27 @@ __device__ __forceinline__ typename Frag<T>::type piece(const T* row,
   return v.f;
 }
 
-template <typename T, int MT, int WAVES>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
     int64_t r, Epilogue e) {
   constexpr int E = 16 / (int)sizeof(T);
   constexpr int CHUNK = LINE / (int)sizeof(T);  // elements of r a line holds
-  __shared__ float sums[WAVES][MT][16][16 + 4];
+  __shared__ float sums[WAVES][16][16 + 4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   // rows past the end repeat the last one; nothing of them is stored
   const T* wrow = w + min(n0 + c, e.n - 1) * ldw;
-  const T* xrow[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-    xrow[i] = x + min((int64_t)i * 16 + c, e.m - 1) * ldx;
+  const T* xrow = x + min((int64_t)c, e.m - 1) * ldx;
 
-  f32x4 acc[MT][1] = {};
+  f32x4 acc[1][1] = {};
   using F = typename Frag<T>::type;
   auto take = [&](int64_t chunk, auto lines, auto whole) {
     constexpr int N = decltype(lines)::value;
     constexpr bool WHOLE = decltype(whole)::value;
-    F wf[N][2][1], xf[N][2][MT];
+    F wf[N][2][1], xf[N][2][1];
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -72,9 +70,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
         const int64_t k =
             (chunk + u * WAVES) * CHUNK + h * (CHUNK / 2) + g * E;
         wf[u][h][0] = piece<T, WHOLE>(wrow, k, r);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          xf[u][h][i] = piece<T, WHOLE>(xrow[i], k, r);
+        xf[u][h][0] = piece<T, WHOLE>(xrow, k, r);
       }
 #pragma unroll
     for (int u = 0; u < N; ++u)
@@ -91,36 +87,27 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_k(
     take(k0, std::integral_constant<int, 1>{}, std::false_type{});
 
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) sums[wave][i][c][g * 4 + q] = acc[i][0][q];
+  for (int q = 0; q < 4; ++q) sums[wave][c][g * 4 + q] = acc[0][0][q];
   __syncthreads();
   const int t = threadIdx.x;
-  if (t < MT * 32) {
+  if (t < 32) {
     const int64_t i = t >> 1, j = n0 + (t & 1) * 8;
     if (i < e.m && j < e.n) {
       float sum[8] = {}, bias[8];
 #pragma unroll 2
       for (int s = 0; s < WAVES; ++s)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          sum[k] += sums[s][i >> 4][i & 15][(t & 1) * 8 + k];
+        for (int k = 0; k < 8; ++k) sum[k] += sums[s][i][(t & 1) * 8 + k];
       load_bias8<T>(e, j, bias);
       finish8<T>(e, i, j, sum, bias);
     }
   }
 }
 
-template <typename T, int MT>
-void launch_few(const DdlProduct* p, hipStream_t s) {
-  few_rows_k<T, MT, 16><<<(unsigned)cdiv(p->n, 16), 1024, 0, s>>>(
-      (const T*)p->a, p->lda, (const T*)p->b, p->ldb, p->r, epilogue_of(p));
-}
-
 template <typename T>
 void run_few(const DdlProduct* p, hipStream_t s) {
-  if (p->m <= 16) launch_few<T, 1>(p, s);
-  else launch_few<T, 2>(p, s);
+  few_rows_k<T, 16><<<(unsigned)cdiv(p->n, 16), 1024, 0, s>>>(
+      (const T*)p->a, p->lda, (const T*)p->b, p->ldb, p->r, epilogue_of(p));
 }
 
 // ---- backward of the activation, bias gradient ------------------------------
@@ -271,7 +258,22 @@ void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
   }
 }
 
-int ddl_few_rows(void) { return 32; }
+// The few-row kernel, and the tiled one with what comes before it, in us.  A
+// block of the former reads its part of W at 28 KB a us, less with more rows
+// of x beside it, and a third of that where 2-byte rows begin anywhere: 16 x
+// 25088 -> 4096 takes 46 us (tiled 34), 1 x 16384 -> 128 20 (10), 16 x 4096 ->
+// 4096 10.9 (12.5), 1 x 2047 -> 1001 10.7 (13.6, of which packing 5).
+bool ddl_few_rows_pay(const DdlProduct* p, bool aligned) {
+  if (p->m > 16 || p->n >= ((int64_t)1 << 26)) return false;  // its grid
+  const float size = p->dtype == 0 ? 4.f : 2.f;
+  const float row = p->r * size, all = row * p->n;
+  float rate = 28e3f / (1.f + 0.8f * p->m / 16.f);
+  if (!aligned && p->dtype != 0) rate /= 3.f;
+  const float rounds = std::ceil(p->n / (16.f * compute_units()));
+  const float few = 1.f + std::max(all / 5.5e6f, rounds * 16.f * row / rate);
+  const float tiled = p->us + (aligned ? 0.f : 5.f + all / 2e6f);
+  return few <= tiled;
+}
 
 void ddl_product_few(const DdlProduct* p, hipStream_t s) {
   switch (p->dtype) {

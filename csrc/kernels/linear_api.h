@@ -38,9 +38,11 @@ struct DdlProduct {
 int64_t ddl_product_plan(DdlProduct* p);
 void ddl_product(const DdlProduct* p, hipStream_t s);
 
-// The same for at most ddl_few_rows() rows, both operands with r contiguous
-// and rows anywhere (any lda, ldb, r and alignment); needs no slabs.
-int ddl_few_rows(void);
+// The same for at most 16 rows, both operands with r contiguous and rows
+// anywhere (any lda, ldb, r and alignment); needs no slabs.  Whether that is
+// estimated to be faster than the planned product; `aligned`: its operands
+// would not have to be packed.
+bool ddl_few_rows_pay(const DdlProduct* p, bool aligned);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
 // dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of

@@ -646,6 +646,10 @@ inline void plan_product(DdlProduct* p) {
   const float units = (float)compute_units();
   p->steps = cdiv(p->r * (p->dtype == 0 ? 4 : 2), LINE);
   p->kind = -1;
+  // what any of them has to move, at 5.5 TB/s
+  const float memory = (p->dtype == 0 ? 4.f : 2.f) / 5.5e6f *
+                       ((float)p->m * p->r + (float)p->n * p->r +
+                        (float)p->m * p->n);
   auto consider = [&](const TileKind& k, int kind) {
     const float tiles = (float)(cdiv(p->m, k.bm) * cdiv(p->n, k.bn));
     for (const int s : SPLITS) {
@@ -659,6 +663,7 @@ inline void plan_product(DdlProduct* p) {
       // many rounds do not end together
       rounds = rounds <= 3.f ? std::ceil(rounds) : rounds + 0.5f;
       float us = rounds * (k.ends + per * step);
+      us = std::max(us, memory);
       if (s > 1) us += 3.f + s * (float)p->m * (float)p->n * 8e-7f;
       if (p->kind < 0 || us < p->us) {
         p->us = us;
