@@ -31,6 +31,8 @@ int code_of(at::ScalarType t) {
   }
 }
 
+constexpr int64_t LIMIT = (int64_t)1 << 29;
+
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // A matrix whose columns are neighbours in memory; its rows may lie anywhere.
@@ -169,7 +171,11 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
   const bool products = k > 0 && (want_dx || want_dw);
   if (act) {
     zc = inner_contiguous(z);
-    if (products) dz = at::empty({m, round_up(n, 8)}, x.options());
+    if (products) {
+      TORCH_CHECK(round_up(n, 8) < reach(x), "the backward pass of ", n,
+                  " outputs: the kernel's offsets reach ", reach(x));
+      dz = at::empty({m, round_up(n, 8)}, x.options());
+    }
   }
   DdlBiasFold fold{};
   at::Tensor partials;
@@ -327,6 +333,10 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
   const bool matrix = x.dim() == 2;
   int64_t rows = 1;
   for (size_t d = 0; d + 1 < shape.size(); ++d) rows *= shape[d];
+  // a grid holds below 2^32 threads, 256 of them take 64 rows or outputs
+  TORCH_CHECK_VALUE(rows < LIMIT && n < LIMIT, "x of ", rows,
+                    " rows and weight of ", n, " outputs: below ", LIMIT,
+                    " of each are supported");
   at::Tensor x2 = matrix ? x : x.reshape({rows, k});
   if (!matrix && residual.has_value()) residual = residual->reshape({rows, n});
   const bool products =

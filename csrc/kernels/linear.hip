@@ -139,45 +139,49 @@ __global__ __launch_bounds__(256) void act_bwd_k(
   __shared__ float part[8][BWD_COLS];
   const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
   const int64_t col_blocks = cdiv(n, BWD_COLS);
-  const int64_t cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks;
-  const int64_t j = cb * BWD_COLS + cg * 8;
   constexpr int TURNS = BWD_ROWS / 8;
-  float v[TURNS][8], q[TURNS][8], sum[8] = {};
-  const int64_t i0 = rb * BWD_ROWS + rg;
+  for (int64_t b = blockIdx.x; b < col_blocks * cdiv(m, BWD_ROWS);
+       b += gridDim.x) {
+    const int64_t cb = b % col_blocks, rb = b / col_blocks;
+    const int64_t j = cb * BWD_COLS + cg * 8;
+    float v[TURNS][8], q[TURNS][8], sum[8] = {};
+    const int64_t i0 = rb * BWD_ROWS + rg;
 #pragma unroll
-  for (int t = 0; t < TURNS; ++t) {  // all loads first
-    const int64_t i = i0 + t * 8;
-    const int64_t end = i < m ? n : 0;  // rows past the end are empty
-    row8(dy + (i < m ? i * lddy : 0), j, end, v[t]);
-    if (act) row8(z + (i < m ? i * ldz : 0), j, end, q[t]);
-  }
-#pragma unroll
-  for (int t = 0; t < TURNS; ++t) {
-    if (act) activate_grad8(v[t], q[t], act);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      // a gradient of NaN behind the row's end would enter the products
-      if (j + k >= n) v[t][k] = 0.f;
-      sum[k] += v[t][k];
+    for (int t = 0; t < TURNS; ++t) {  // all loads first
+      const int64_t i = i0 + t * 8;
+      const int64_t end = i < m ? n : 0;  // rows past the end are empty
+      row8(dy + (i < m ? i * lddy : 0), j, end, v[t]);
+      if (act) row8(z + (i < m ? i * ldz : 0), j, end, q[t]);
     }
-    const int64_t i = i0 + t * 8;
-    if (dz && i < m && j < lddz) {  // lddz is a multiple of 8
-      Vec8<T> o;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(v[t][k]);
-      store8(dz + i * lddz + j, o);
+    for (int t = 0; t < TURNS; ++t) {
+      if (act) activate_grad8(v[t], q[t], act);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        // a gradient of NaN behind the row's end would enter the products
+        if (j + k >= n) v[t][k] = 0.f;
+        sum[k] += v[t][k];
+      }
+      const int64_t i = i0 + t * 8;
+      if (dz && i < m && j < lddz) {  // lddz is a multiple of 8
+        Vec8<T> o;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(v[t][k]);
+        store8(dz + i * lddz + j, o);
+      }
     }
-  }
-  if (!partials) return;
+    if (!partials) continue;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) part[rg][cg * 8 + k] = sum[k];
-  __syncthreads();
-  const int64_t col = cb * BWD_COLS + threadIdx.x;
-  if (col < n) {
-    float total = 0.f;
+    for (int k = 0; k < 8; ++k) part[rg][cg * 8 + k] = sum[k];
+    __syncthreads();
+    const int64_t col = cb * BWD_COLS + threadIdx.x;
+    if (col < n) {
+      float total = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) total += part[k][threadIdx.x];
-    partials[rb * n + col] = total;
+      for (int k = 0; k < 8; ++k) total += part[k][threadIdx.x];
+      partials[rb * n + col] = total;
+    }
+    __syncthreads();  // before the next turn's sums
   }
 }
 
@@ -222,8 +226,8 @@ template <typename T, typename Z>
 void run_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz,
                  void* dz, int64_t lddz, int64_t m, int64_t n, int act,
                  float* partials, hipStream_t s) {
-  const unsigned blocks =
-      (unsigned)(cdiv(m, BWD_ROWS) * cdiv(n, BWD_COLS));
+  const unsigned blocks = (unsigned)std::min<int64_t>(
+      cdiv(m, BWD_ROWS) * cdiv(n, BWD_COLS), 1 << 20);
   act_bwd_k<T, Z><<<blocks, 256, 0, s>>>((const T*)dy, lddy, (const Z*)z, ldz,
                                          (T*)dz, lddz, m, n, act, partials);
 }

@@ -164,6 +164,8 @@ class Linear(nn.Module):
     epilogue (``functional.linear_act``); without either this is a plain
     library product."""
 
+    activation = "none"  # modules pickled without one
+
     def __init__(self, in_features, out_features, bias=True,
                  activation="none"):
         super().__init__()

@@ -405,7 +405,12 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, sd):
         """Exact-dtype restore, as FusedSGD's; the state tensors of ``sd``
-        are taken over without a copy where they are on the right device."""
+        are taken over without a copy where they are on the right device.
+        The state of a ``torch.optim.AdamW`` is understood too."""
+        for group in sd["param_groups"]:
+            for option in ("amsgrad", "maximize"):
+                if group.get(option):
+                    raise ValueError(f"{option} is not supported")
         _restore_exact(self, sd)
         for group in self.param_groups:
             group["betas"] = tuple(group["betas"])
@@ -435,8 +440,12 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise ValueError("8-bit moments belong to the memory layout "
                                  "that they were saved in")
             st[name] = torch.empty_like(p, dtype=t.dtype).copy_(t)
+        if bits == 32:  # torch holds the moments in the parameter's dtype
+            for name in ("exp_avg", "exp_avg_sq"):
+                st[name] = st[name].to(torch.float32)
         if not torch.is_tensor(st["step"]):
-            st["step"] = torch.tensor(float(st["step"]), device=p.device)
+            st["step"] = torch.tensor(float(st["step"]))
+        st["step"] = st["step"].to(p.device, torch.float32)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -491,12 +500,16 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step_gpu(self):
         if self._plans is None:
             self._build_plans()
-        missing = False
+        missing = []  # parameters with their first gradient
         for plan, group, members in self._plans:
-            for i in plan.collect():  # the first gradient of a parameter
-                self._init_state(members[i], group["state_bits"])
-                missing = True
+            missing += [(i, members, group["state_bits"])
+                        for i in plan.collect()]
         if missing:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("take a step before capturing one: a "
+                                   "replay would begin with new states")
+            for i, members, bits in missing:
+                self._init_state(members[i], bits)
             self._build_plans()
             for plan, _, _ in self._plans:
                 plan.collect()

@@ -401,6 +401,42 @@ def test_captured_step_counts_on(bits):
 
 
 @gpu
+def test_first_step_is_not_captured():
+    params = make([100], torch.float32, "cuda")
+    opt = FusedAdamW(params)
+    graph = torch.cuda.CUDAGraph()
+    before = params[0].detach().clone()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(graph):
+            params[0].grad.mul_(2.0)
+            opt.step()
+    assert "step" not in opt.state[params[0]]
+    opt.step()
+    assert not torch.equal(params[0], before)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_takes_over_the_state_of_torch(device, dtype):
+    params = make([300, 5], dtype, device)
+    ref = torch.optim.AdamW(params, lr=1e-2)
+    ref.step()
+    opt = FusedAdamW(params)
+    opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 1e-2
+    before = opt.state[params[0]]["exp_avg"].clone()
+    opt.step()
+    st = opt.state[params[0]]
+    assert float(st["step"]) == 2 and st["exp_avg"].dtype == torch.float32
+    want = 0.9 * before.double() + 0.1 * params[0].grad.double()
+    assert (st["exp_avg"].double() - want).abs().max() <= 4 * U * 0.1
+    ref.param_groups[0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(ref.state_dict())
+
+
+@gpu
 def test_step_on_another_stream():
     params = make([100000], torch.bfloat16, "cuda")
     twins = make([100000], torch.bfloat16, "cuda")

@@ -331,6 +331,15 @@ def test_values_that_are_not_finite_stay_in_their_row(device, dtype):
     assert torch.equal(y[keep], clean[keep])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_small_halves_are_not_flushed(device):
+    """float16's smallest numbers, 2^-24 apart below 2^-14, count."""
+    for m in (3, 100):
+        x = torch.full((m, 64), 2.0 ** -22, dtype=torch.float16, device=device)
+        w = torch.ones(24, 64, dtype=torch.float16, device=device)
+        assert (DF.linear_act(x, w) == 2.0 ** -16).all()
+
+
 @gpu
 def test_offsets_past_32_bits():
     n = (1 << 25) + 8  # 2^31 elements and some, 4 GiB
@@ -468,3 +477,14 @@ def test_refused_on_the_gpu():
     (g,) = torch.autograd.grad(y.sum(), w, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+    # more rows than a grid holds, more columns than offsets reach
+    with pytest.raises(ValueError, match="rows"):
+        DF.linear_act(x[:1].expand(1 << 29, 8), w)
+    wide = torch.zeros(1, 1, device="cuda").expand(20, (1 << 22) + 8)
+    with pytest.raises(RuntimeError, match="reach"):
+        DF.linear_act(wide, wide)
+    many = torch.zeros((1 << 22) + 8, 8, dtype=torch.bfloat16, device="cuda",
+                       requires_grad=True)
+    y = DF.linear_act(x.bfloat16(), many, None, "relu")
+    with pytest.raises(RuntimeError, match="reach"):
+        y.sum().backward()
