@@ -39,10 +39,11 @@ constexpr int THREADS = 256;
 constexpr int MOMENT_BLOCK = DDL_MOMENT_BLOCK;
 static_assert(MOMENT_BLOCK == 32 * 8, "half a wave holds a block");
 
-// Kernel arguments hold at most 4 KiB.
-constexpr int MAX_T32 = 64;
-constexpr int MAX_T8 = 48;
-constexpr int MAX_NORM = 160;
+// Kernel arguments hold at most 4 KiB.  A tensor's length is told by its
+// blocks and by what its last block lacks.
+constexpr int MAX_T32 = 84;
+constexpr int MAX_T8 = 62;
+constexpr int MAX_NORM = 270;
 constexpr int MAX_PREP = 192;
 
 struct Scalars {  // per tensor, written by prepare_k
@@ -58,7 +59,6 @@ struct T32 {
   float* w;
   float* m;
   float* v;
-  int64_t n;
 };
 
 struct T8 : T32 {
@@ -66,23 +66,31 @@ struct T8 : T32 {
   float* vs;
 };
 
+struct TG {
+  void* g;
+};
+
 template <typename Row, int MAX> struct Args {
   Row t[MAX];
-  int first[MAX];       // first block of each tensor
+  int first[MAX + 1];   // first block of each tensor, and the end
+  uint16_t lacks[MAX];  // elements that the last block is short of a chunk
   uint8_t aligned[MAX]; // every pointer of the tensor takes 16-byte accesses
   int count;
   int chunk;            // elements a block
+
+  // Elements of this block of tensor i.
+  __device__ __forceinline__ void range(int i, int64_t& begin,
+                                        int64_t& end) const {
+    const int block = (int)blockIdx.x - first[i];
+    begin = (int64_t)block * chunk;
+    end = begin + chunk -
+          ((int)blockIdx.x + 1 == first[i + 1] ? lacks[i] : 0);
+  }
 };
+using NormArgs = Args<TG, MAX_NORM>;
 static_assert(sizeof(Args<T32, MAX_T32>) < 4000, "kernel argument limit");
 static_assert(sizeof(Args<T8, MAX_T8>) < 4000, "kernel argument limit");
-
-struct NormArgs {
-  void* g[MAX_NORM];
-  int64_t n[MAX_NORM];
-  int first[MAX_NORM];
-  int count;
-  int chunk;
-};
+static_assert(sizeof(NormArgs) < 4080, "kernel argument limit");
 
 struct PrepArgs {
   float* step[MAX_PREP];
@@ -189,8 +197,8 @@ __global__ __launch_bounds__(THREADS) void adamw32_k(
   const Scalars s = ws[ti];
   Update up{c, coef ? c.grad_mul * *coef : c.grad_mul, s.step_size,
             s.inv_sqrt_c2};
-  const int64_t begin = (int64_t)(blockIdx.x - a.first[ti]) * a.chunk;
-  const int64_t end = min(t.n, begin + a.chunk);
+  int64_t begin, end;
+  a.range(ti, begin, end);
   T* p = (T*)t.p;
   const T* grad = (const T*)t.g;
   if (a.aligned[ti]) {
@@ -288,8 +296,8 @@ __global__ __launch_bounds__(THREADS) void adamw8_k(
   const Scalars s = ws[ti];
   Update up{c, coef ? c.grad_mul * *coef : c.grad_mul, s.step_size,
             s.inv_sqrt_c2};
-  const int64_t begin = (int64_t)(blockIdx.x - a.first[ti]) * a.chunk;
-  const int64_t end = min(t.n, begin + a.chunk);
+  int64_t begin, end;
+  a.range(ti, begin, end);
   T* p = (T*)t.p;
   const T* grad = (const T*)t.g;
   uint8_t* mc = (uint8_t*)t.m;
@@ -385,10 +393,10 @@ template <typename T>
 __global__ __launch_bounds__(THREADS) void grad_norm_k(NormArgs a,
                                                        double* partials) {
   const int ti = find_tensor(a.first, a.count, blockIdx.x);
-  const T* g = (const T*)a.g[ti];
-  const int64_t begin = (int64_t)(blockIdx.x - a.first[ti]) * a.chunk;
-  const int64_t end = min(a.n[ti], begin + a.chunk);
-  const bool aligned = ((uintptr_t)g & 15) == 0;
+  const T* g = (const T*)a.t[ti].g;
+  int64_t begin, end;
+  a.range(ti, begin, end);
+  const bool aligned = a.aligned[ti];
   double sum = 0.0;
   auto add = [&](const Vec8<T>& x) {
 #pragma unroll
@@ -422,10 +430,10 @@ __global__ __launch_bounds__(THREADS) void grad_scale_k(
   const float k = *coef;
   if (k == 1.f) return;
   const int ti = find_tensor(a.first, a.count, blockIdx.x);
-  T* g = (T*)a.g[ti];
-  const int64_t begin = (int64_t)(blockIdx.x - a.first[ti]) * a.chunk;
-  const int64_t end = min(a.n[ti], begin + a.chunk);
-  const bool aligned = ((uintptr_t)g & 15) == 0;
+  T* g = (T*)a.t[ti].g;
+  int64_t begin, end;
+  a.range(ti, begin, end);
+  const bool aligned = a.aligned[ti];
   if (aligned) {
     for (int64_t i = begin + threadIdx.x * 8; i + 8 <= end;
          i += THREADS * 8) {
@@ -463,23 +471,27 @@ bool takes16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Hands `launch` the tensors in groups of at most MAX, with the blocks that
 // each group needs and the place of its first tensor.
-template <typename A, int MAX, typename Size, typename Fill, typename Launch>
-void in_groups(int64_t count, int chunk, Size size, Fill fill, Launch launch) {
-  A a;
+template <typename Row, int MAX, typename Tensor, typename Fill,
+          typename Launch>
+void in_groups(const Tensor* t, int64_t count, Fill fill, Launch launch) {
+  Args<Row, MAX> a;
   a.count = 0;
-  a.chunk = chunk;
+  a.chunk = chunk_of(total_of(t, count));
   int64_t blocks = 0, start = 0;
   auto flush = [&](int64_t next) {
+    a.first[a.count] = (int)blocks;
     if (blocks) launch(a, (int)blocks, start);
     a.count = 0;
     blocks = 0;
     start = next;
   };
   for (int64_t i = 0; i < count; ++i) {
-    const int64_t more = cdiv(size(i), chunk);
+    const int64_t more = cdiv(t[i].n, a.chunk);
     if (a.count == MAX || blocks + more > MAX_BLOCKS) flush(i);
-    fill(a, a.count, i);
-    a.first[a.count++] = (int)blocks;
+    a.first[a.count] = (int)blocks;
+    a.lacks[a.count] = (uint16_t)(more * a.chunk - t[i].n);
+    a.aligned[a.count] = fill(a.t[a.count], t[i]);
+    ++a.count;
     blocks += more;
   }
   flush(count);
@@ -496,38 +508,33 @@ template <typename T, bool MASTER>
 void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
                int bits, const Scalars* ws, const float* coef,
                hipStream_t s) {
-  const int chunk = chunk_of(total_of(t, count));
-  auto size = [&](int64_t i) { return t[i].n; };
-  auto common = [&](T32& r, int64_t i) {
-    r.p = t[i].p;
-    r.g = t[i].g;
-    r.w = t[i].w;
-    r.m = (float*)t[i].m;
-    r.v = (float*)t[i].v;
-    r.n = t[i].n;
-    return (!MASTER || takes16(r.p)) && takes16(r.g) && takes16(r.w);
+  auto common = [](T32& r, const DdlAdamTensor& t) {
+    r.p = t.p;
+    r.g = t.g;
+    r.w = t.w;
+    r.m = (float*)t.m;
+    r.v = (float*)t.v;
+    return (!MASTER || takes16(t.p)) && takes16(t.g) && takes16(t.w);
   };
   if (bits == 32) {
-    using A = Args<T32, MAX_T32>;
-    in_groups<A, MAX_T32>(count, chunk, size,
-        [&](A& a, int k, int64_t i) {
-          a.aligned[k] = common(a.t[k], i) && takes16(t[i].m) &&
-                         takes16(t[i].v);
+    in_groups<T32, MAX_T32>(
+        t, count,
+        [&](T32& r, const DdlAdamTensor& t) {
+          return common(r, t) && takes16(t.m) && takes16(t.v);
         },
-        [&](const A& a, int blocks, int64_t at) {
+        [&](const auto& a, int blocks, int64_t at) {
           adamw32_k<T, MASTER><<<blocks, THREADS, 0, s>>>(a, c, ws + at, coef);
         });
   } else {
-    using A = Args<T8, MAX_T8>;
-    in_groups<A, MAX_T8>(count, chunk, size,
-        [&](A& a, int k, int64_t i) {
-          a.aligned[k] = common(a.t[k], i) &&
-                         ((uintptr_t)t[i].m & 7) == 0 &&
-                         ((uintptr_t)t[i].v & 7) == 0;
-          a.t[k].ms = t[i].ms;
-          a.t[k].vs = t[i].vs;
+    in_groups<T8, MAX_T8>(
+        t, count,
+        [&](T8& r, const DdlAdamTensor& t) {
+          r.ms = t.ms;
+          r.vs = t.vs;
+          return common(r, t) && ((uintptr_t)t.m & 7) == 0 &&
+                 ((uintptr_t)t.v & 7) == 0;
         },
-        [&](const A& a, int blocks, int64_t at) {
+        [&](const auto& a, int blocks, int64_t at) {
           adamw8_k<T, MASTER><<<blocks, THREADS, 0, s>>>(a, c, ws + at, coef);
         });
   }
@@ -535,11 +542,11 @@ void run_adamw(const DdlAdamTensor* t, int64_t count, const Consts& c,
 
 template <typename Launch>
 void norm_groups(const DdlGradTensor* t, int64_t count, Launch launch) {
-  in_groups<NormArgs, MAX_NORM>(count, chunk_of(total_of(t, count)),
-      [&](int64_t i) { return t[i].n; },
-      [&](NormArgs& a, int k, int64_t i) {
-        a.g[k] = t[i].g;
-        a.n[k] = t[i].n;
+  in_groups<TG, MAX_NORM>(
+      t, count,
+      [](TG& r, const DdlGradTensor& t) {
+        r.g = t.g;
+        return takes16(t.g);
       },
       launch);
 }

@@ -494,6 +494,18 @@ def test_clip_matches_64_bits(device, dtype, offset, max_norm):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_clip_of_more_tensors_than_a_launch_takes(device):
+    params = make([(41 * i) % 97 for i in range(600)], torch.float32, device)
+    grads = [p.grad.clone() for p in params]
+    norm = clip_grad_norm_(params, 0.1)
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    assert abs(float(norm) - want) <= 2 * U * want
+    for p, g in zip(params, grads):
+        ref = g.double() * (0.1 / (want + 1e-6))
+        assert ((p.grad.double() - ref).abs() <= ref.abs() * 8 * U).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_clip_edges(device):
     p = make([5], torch.float32, device)[0]
     p.grad.zero_()
