@@ -168,6 +168,17 @@ def test_every_tile(dtype, shape):
     run_case(*shape, dtype, "cuda", "silu")
 
 
+@gpu
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 5800),
+                                        (torch.float16, 5801),
+                                        (torch.float32, 4100)])
+def test_outputs_stored_past_the_caches(dtype, size):
+    """64 MB and more: a forward and a weight gradient, lines that start at
+    even and at odd multiples of the element."""
+    run_case(size, 24, 5802, dtype, "cuda", "silu")
+    run_case(40, 5801, size, dtype, "cuda", "relu", residual=False)
+
+
 def test_every_tile_is_planned():
     ext = load_kernels_ext(required=False)
     if ext is None:
