@@ -180,7 +180,7 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
   DdlBiasFold fold{};
   at::Tensor partials;
   if (want_db) {
-    fold.chunks = ddl_bias_chunks(m);
+    fold.chunks = ddl_bias_chunks(m, n);
     fold.n = n;
     partials = at::empty({fold.chunks * n}, x.options().dtype(at::kFloat));
     fold.partials = partials.data_ptr<float>();

@@ -112,8 +112,21 @@ void run_few(const DdlProduct* p, hipStream_t s) {
 
 // ---- backward of the activation, bias gradient ------------------------------
 
-constexpr int BWD_ROWS = 16;   // rows a block sums
-constexpr int BWD_COLS = 256;  // 32 threads of 8 columns
+// 256 threads take 8 columns each: LANES of them a row, all rows of a turn
+// twice.  64 columns a block where there are no more, 256 otherwise.
+constexpr int BWD_NARROW = 8, BWD_WIDE = 32;
+
+// Rows that a block sums: one turn where there are few, as many turns as leave
+// four blocks to a compute unit where there are many, since the bias
+// gradient's fold reads a number a column of each block.  1048576 x 64 -> 8
+// with its gradients takes 359 us so; 1056 with 16 rows a block and 32 lanes a
+// row at all sizes.
+inline int64_t bwd_rows(int64_t m, int64_t n) {
+  const int64_t lanes = n <= BWD_NARROW * 8 ? BWD_NARROW : BWD_WIDE;
+  const int64_t turn = 2 * (256 / lanes);
+  const int64_t blocks = cdiv(n, lanes * 8) * cdiv(m, turn);
+  return turn * std::max<int64_t>(1, cdiv(blocks, 4 * compute_units()));
+}
 
 // Elements j..j+7 of a row of n, zeros behind its end; it may begin anywhere.
 template <typename T>
@@ -131,30 +144,30 @@ __device__ __forceinline__ void row8(const T* row, int64_t j, int64_t n,
   for (int k = 0; k < 8; ++k) out[k] = to_f32(r[k]);
 }
 
-template <typename T, typename Z>
+template <typename T, typename Z, int LANES>
 __global__ __launch_bounds__(256) void act_bwd_k(
     const T* __restrict__ dy, int64_t lddy, const Z* __restrict__ z,
     int64_t ldz, T* __restrict__ dz, int64_t lddz, int64_t m, int64_t n,
-    int act, float* __restrict__ partials) {
-  __shared__ float part[8][BWD_COLS];
-  const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
-  const int64_t col_blocks = cdiv(n, BWD_COLS);
-  constexpr int TURNS = BWD_ROWS / 8;
-  for (int64_t b = blockIdx.x; b < col_blocks * cdiv(m, BWD_ROWS);
-       b += gridDim.x) {
-    const int64_t cb = b % col_blocks, rb = b / col_blocks;
-    const int64_t j = cb * BWD_COLS + cg * 8;
-    float v[TURNS][8], q[TURNS][8], sum[8] = {};
-    const int64_t i0 = rb * BWD_ROWS + rg;
+    int64_t rows, int act, float* __restrict__ partials) {
+  constexpr int GROUPS = 256 / LANES, COLS = LANES * 8;
+  __shared__ float part[GROUPS][COLS];
+  const int cg = threadIdx.x % LANES, rg = threadIdx.x / LANES;
+  const int64_t col_blocks = cdiv(n, COLS);
+  const int64_t cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks;
+  const int64_t j = cb * COLS + cg * 8;
+  const int64_t end_row = min(m, (rb + 1) * rows);
+  float sum[8] = {};
+  for (int64_t i0 = rb * rows + rg; i0 < end_row; i0 += 2 * GROUPS) {
+    float v[2][8], q[2][8];
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {  // all loads first
-      const int64_t i = i0 + t * 8;
-      const int64_t end = i < m ? n : 0;  // rows past the end are empty
-      row8(dy + (i < m ? i * lddy : 0), j, end, v[t]);
-      if (act) row8(z + (i < m ? i * ldz : 0), j, end, q[t]);
+    for (int t = 0; t < 2; ++t) {  // all loads first
+      const int64_t i = i0 + t * GROUPS;
+      const int64_t end = i < end_row ? n : 0;  // rows past the end are empty
+      row8(dy + (i < end_row ? i * lddy : 0), j, end, v[t]);
+      if (act) row8(z + (i < end_row ? i * ldz : 0), j, end, q[t]);
     }
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {
+    for (int t = 0; t < 2; ++t) {
       if (act) activate_grad8(v[t], q[t], act);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -162,26 +175,25 @@ __global__ __launch_bounds__(256) void act_bwd_k(
         if (j + k >= n) v[t][k] = 0.f;
         sum[k] += v[t][k];
       }
-      const int64_t i = i0 + t * 8;
-      if (dz && i < m && j < lddz) {  // lddz is a multiple of 8
+      const int64_t i = i0 + t * GROUPS;
+      if (dz && i < end_row && j < lddz) {  // lddz is a multiple of 8
         Vec8<T> o;
 #pragma unroll
         for (int k = 0; k < 8; ++k) o.v[k] = from_f32<T>(v[t][k]);
         store8(dz + i * lddz + j, o);
       }
     }
-    if (!partials) continue;
+  }
+  if (!partials) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) part[rg][cg * 8 + k] = sum[k];
-    __syncthreads();
-    const int64_t col = cb * BWD_COLS + threadIdx.x;
-    if (col < n) {
-      float total = 0.f;
+  for (int k = 0; k < 8; ++k) part[rg][cg * 8 + k] = sum[k];
+  __syncthreads();
+  const int64_t col = cb * COLS + threadIdx.x;
+  if (threadIdx.x < COLS && col < n) {
+    float total = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) total += part[k][threadIdx.x];
-      partials[rb * n + col] = total;
-    }
-    __syncthreads();  // before the next turn's sums
+    for (int k = 0; k < GROUPS; ++k) total += part[k][threadIdx.x];
+    partials[rb * n + col] = total;
   }
 }
 
@@ -226,10 +238,16 @@ template <typename T, typename Z>
 void run_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz,
                  void* dz, int64_t lddz, int64_t m, int64_t n, int act,
                  float* partials, hipStream_t s) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(
-      cdiv(m, BWD_ROWS) * cdiv(n, BWD_COLS), 1 << 20);
-  act_bwd_k<T, Z><<<blocks, 256, 0, s>>>((const T*)dy, lddy, (const Z*)z, ldz,
-                                         (T*)dz, lddz, m, n, act, partials);
+  const int64_t rows = bwd_rows(m, n), chunks = cdiv(m, rows);
+  auto launch = [&](auto kernel, int lanes) {
+    kernel<<<(unsigned)(chunks * cdiv(n, lanes * 8)), 256, 0, s>>>(
+        (const T*)dy, lddy, (const Z*)z, ldz, (T*)dz, lddz, m, n, rows, act,
+        partials);
+  };
+  if (n <= BWD_NARROW * 8)
+    launch(act_bwd_k<T, Z, BWD_NARROW>, BWD_NARROW);
+  else
+    launch(act_bwd_k<T, Z, BWD_WIDE>, BWD_WIDE);
 }
 
 }  // namespace
@@ -287,7 +305,9 @@ void ddl_product_few(const DdlProduct* p, hipStream_t s) {
   }
 }
 
-int64_t ddl_bias_chunks(int64_t m) { return cdiv(m, BWD_ROWS); }
+int64_t ddl_bias_chunks(int64_t m, int64_t n) {
+  return cdiv(m, bwd_rows(m, n));
+}
 
 void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
                  int64_t ldz, void* dz, int64_t lddz, int64_t m, int64_t n,

@@ -46,10 +46,10 @@ bool ddl_few_rows_pay(const DdlProduct* p, bool aligned);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
 // dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of
-// 8), and the column sums of dz before its rounding, of 16 rows each: partials
-// holds ddl_bias_chunks(m) * n floats.  z is float32 (z_f32), or for act 1 the
+// 8), and the column sums of dz before its rounding, of some rows each: partials
+// holds ddl_bias_chunks(m, n) * n floats.  z is float32 (z_f32), or for act 1 the
 // output in the tensors' dtype.  dz or partials may be null.
-int64_t ddl_bias_chunks(int64_t m);
+int64_t ddl_bias_chunks(int64_t m, int64_t n);
 void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
                  int64_t ldz, void* dz, int64_t lddz, int64_t m, int64_t n,
                  int act, int dtype, float* partials, hipStream_t s);

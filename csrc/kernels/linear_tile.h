@@ -563,7 +563,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
 }
 
 // The fold of act_bwd_k's partial sums: FOLD_COLS columns a block of 256.
-constexpr int FOLD_COLS = 32;
+constexpr int FOLD_COLS = 16;
 
 template <typename T>
 __device__ __forceinline__ void fold_bias(const DdlBiasFold& f, int64_t block,
@@ -572,9 +572,9 @@ __device__ __forceinline__ void fold_bias(const DdlBiasFold& f, int64_t block,
   double* part = reinterpret_cast<double*>(smem);
   const int col = threadIdx.x % FOLD_COLS, lane = threadIdx.x / FOLD_COLS;
   const int64_t j = block * FOLD_COLS + col;
-  double sum = 0.0;  // as many chunks as there are rows / 16
+  double sum = 0.0;
   if (j < f.n)
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t c = lane; c < f.chunks; c += LANES)
       sum += f.partials[c * f.n + j];
   part[threadIdx.x] = sum;

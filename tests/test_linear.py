@@ -147,6 +147,16 @@ def test_larger(shape, dtype):
     run_case(*shape, dtype, "cuda", "gelu" if shape[0] % 2 else "relu")
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(140003, 8, 9), (140001, 3, 1),
+                                   (40003, 16, 200), (33000, 8, 513),
+                                   (300, 40, 64), (300, 40, 65)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_bias_gradient_over_many_rows(shape, dtype, act):
+    run_case(*shape, dtype, "cuda", act, residual=False)
+
+
 # sizes that reach every tile of the kernel in every product, and split ones
 PLANNED = {
     torch.bfloat16: [(2056, 264, 4104), (2056, 4104, 136), (136, 4104, 2056),
