@@ -6,8 +6,11 @@
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "kernels/linear_api.h"
 
@@ -294,6 +297,22 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
   }
 };
 
+// A leaf whose gradient an eager graph of the default stream still waits for
+// ties a captured backward pass to that stream, which cannot be captured: the
+// engine's thread would end the process.
+void check_capture(const at::Tensor& t, const char* name) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(!stream.has_value() ||
+                  stream->id() != c10::hip::getDefaultHIPStream(
+                                      t.device().index()).id(),
+              "captured while an eager graph that ", name,
+              " is a leaf of lives on the default stream: drop its outputs "
+              "before the capture, or run it on another stream");
+}
+
 // functional.linear_act on a GPU.
 at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
                       const Maybe& bias, int64_t act, Maybe residual) {
@@ -305,11 +324,21 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "x ends in ", k,
                     " features, its shape is ", x.sizes());
   code_of(x.scalar_type());
+  const bool dual = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
+  auto plain = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(!t.is_neg(), name, " is a lazy negation: call "
+                      "resolve_neg() first");
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual || !t._fw_grad(0).defined(), name,
+                                " carries a tangent: linear_act has no "
+                                "forward-mode derivative");
+  };
+  plain(x, "x");
   auto like = [&](const at::Tensor& t, const char* name) {
     TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type() &&
                          t.device() == x.device(),
                      name, " is ", t.scalar_type(), " on ", t.device(),
                      ", x is ", x.scalar_type(), " on ", x.device());
+    plain(t, name);
   };
   like(w, "weight");
   if (bias.has_value()) {
@@ -319,6 +348,7 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
   }
   auto shape = x.sizes().vec();
   shape.back() = n;
+  const at::Tensor given = residual.value_or(at::Tensor());
   if (residual.has_value()) {
     like(*residual, "residual");
     bool ok = residual->dim() <= (int64_t)shape.size();
@@ -346,6 +376,14 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
       products || (residual.has_value() && residual->requires_grad());
   at::Tensor y;
   if (any && c10::GradMode::is_enabled()) {
+    c10::DeviceGuard guard(x.device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+        c10::hip::CaptureStatus::None) {
+      check_capture(x, "x");
+      check_capture(w, "weight");
+      if (bias.has_value()) check_capture(*bias, "bias");
+      check_capture(given, "residual");
+    }
     y = LinearAct::apply(x2, w, bias, residual, act, products);
   } else {
     at::AutoDispatchBelowADInplaceOrView below;

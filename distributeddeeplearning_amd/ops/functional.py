@@ -461,6 +461,10 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     "silu".  Sums, bias, activation and residual are computed in float32 and
     rounded once.  Differentiable once in every tensor; the backward pass
     rounds the activation's gradient to the inputs' dtype before its products.
+
+    A captured call raises where a tensor is a leaf of an eager graph that is
+    still alive on the default stream: its backward pass would have to wait
+    for that stream.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, not "

@@ -509,3 +509,54 @@ def test_refused_on_the_gpu():
     y = DF.linear_act(x.bfloat16(), many, None, "relu")
     with pytest.raises(RuntimeError, match="reach"):
         y.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("leaf", ["x", "weight", "bias", "residual"])
+def test_capture_beside_a_live_eager_graph_is_refused(leaf):
+    t = {"x": torch.randn(3, 8, device="cuda"),
+         "weight": torch.randn(5, 8, device="cuda"),
+         "bias": torch.randn(5, device="cuda"),
+         "residual": torch.randn(3, 5, device="cuda")}
+    t[leaf].requires_grad_(True)
+    alive = DF.linear_act(**t, activation="relu")
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match=f"{leaf} is a leaf"):
+        with torch.cuda.graph(graph):
+            DF.linear_act(**t, activation="relu")
+    with torch.no_grad():  # no backward pass, nothing to refuse
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = DF.linear_act(**t, activation="relu")
+    want = alive.detach().clone()
+    del alive
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    y = DF.linear_act(**t, activation="relu")
+    y.sum().backward()
+    want = t[leaf].grad.clone()
+    del y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t[leaf].grad = None
+        DF.linear_act(**t, activation="relu").sum().backward()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(t[leaf].grad, want)
+
+
+@gpu
+def test_tensors_that_are_not_what_lies_in_memory_are_refused():
+    x = torch.randn(3, 8, device="cuda")
+    w = torch.randn(5, 8, device="cuda")
+    c = torch.randn(3, 8, device="cuda", dtype=torch.complex64)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        DF.linear_act(torch.imag(c.conj()), w)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        with pytest.raises(NotImplementedError, match="weight"):
+            DF.linear_act(x, dual)
+        assert DF.linear_act(x, w).shape == (3, 5)
