@@ -296,8 +296,8 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
                       double max_norm) {
   std::vector<NormList> lists(3);
   for (int i = 0; i < 3; ++i) lists[i].dtype = i;
-  std::unordered_set<const void*> seen;
-  seen.reserve(2 * params.size());
+  std::vector<std::pair<const char*, const char*>> places;
+  places.reserve(params.size());
   c10::optional<c10::Device> device;
   for (const auto& p : params) {
     const at::Tensor& g = p.grad();
@@ -309,10 +309,14 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     TORCH_CHECK(dense(g), "a gradient is not dense in memory");
     const int dtype = code_of(g.scalar_type());
     if (g.numel() == 0) continue;
-    TORCH_CHECK(seen.insert(g.const_data_ptr()).second,
-                "a gradient appears twice");
     lists[dtype].rows.push_back(DdlGradTensor{g.data_ptr(), g.numel()});
+    const char* start = static_cast<const char*>(g.const_data_ptr());
+    places.emplace_back(start, start + g.nbytes());
   }
+  std::sort(places.begin(), places.end());
+  for (size_t i = 1; i < places.size(); ++i)
+    TORCH_CHECK(places[i - 1].second <= places[i].first,
+                "a gradient appears twice, or two share memory");
   TORCH_CHECK(device.has_value(), "no gradients");
   c10::DeviceGuard guard(*device);
   Norm norm = norm_of(lists, *device, grad_mul, max_norm);

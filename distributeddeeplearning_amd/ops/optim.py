@@ -474,8 +474,20 @@ class FusedAdamW(torch.optim.Optimizer):
             self._step_cpu()
         return loss
 
+    def _check_overlap(self):
+        """Tensors of one launch are updated at the same time."""
+        places = sorted(
+            (p.device.index, p.data_ptr(), p.numel() * p.element_size())
+            for g in self.param_groups for p in g["params"]
+            if p.is_cuda and p.numel()
+            and (p.grad is not None or p in self.state))
+        for (dev, at, size), (dev2, at2, _) in zip(places, places[1:]):
+            if dev == dev2 and at + size > at2:
+                raise ValueError("two parameters with gradients share memory")
+
     def _build_plans(self):
         ext = load_kernels_ext()
+        self._check_overlap()
         self._plans = []
         index = 0
         for group in self.param_groups:

@@ -611,3 +611,25 @@ def test_refused_on_the_gpu():
     a.grad = torch.zeros(1, device="cuda").expand(5)
     with pytest.raises(RuntimeError, match="dense"):
         clip_grad_norm_([a], 1.0)
+
+
+@gpu
+def test_tensors_that_share_memory_are_refused():
+    base = torch.randn(100, device="cuda")
+    a, b, c = (torch.nn.Parameter(base[i:i + 50]) for i in (0, 49, 50))
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW([a, b]).step()
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW([{"params": [b]}, {"params": [a], "lr": 0.1}]).step()
+    before = base.clone()
+    FusedAdamW([a, c], weight_decay=0.0, lr=0.5).step()
+    assert (base < before).all()
+    b.grad = None  # not updated
+    FusedAdamW([a, b, c]).step()
+    a.grad, c.grad = base[:50], base[49:99]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_([a, c], 1.0)
+    c.grad = base[50:]
+    clip_grad_norm_([a, c], 1.0)
