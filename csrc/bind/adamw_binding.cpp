@@ -320,10 +320,12 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
   TORCH_CHECK(device.has_value(), "no gradients");
   c10::DeviceGuard guard(*device);
   Norm norm = norm_of(lists, *device, grad_mul, max_norm);
-  ddl_grad_norm_fold(&norm.fold, stream_now());
+  const bool fold =
+      norm.fold.blocks > 0 && norm.fold.blocks <= DDL_FOLD_IN_SCALE;
+  if (!fold) ddl_grad_norm_fold(&norm.fold, stream_now());
   for (const auto& l : lists)
-    ddl_grad_scale(l.rows.data(), (int64_t)l.rows.size(), l.dtype,
-                   norm.fold.coef, stream_now());
+    ddl_grad_scale(l.rows.data(), (int64_t)l.rows.size(), l.dtype, &norm.fold,
+                   fold, stream_now());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return norm.norm;
 }

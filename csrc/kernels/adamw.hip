@@ -43,7 +43,7 @@ static_assert(MOMENT_BLOCK == 32 * 8, "half a wave holds a block");
 // blocks and by what its last block lacks.
 constexpr int MAX_T32 = 84;
 constexpr int MAX_T8 = 62;
-constexpr int MAX_NORM = 270;
+constexpr int MAX_NORM = 266;
 constexpr int MAX_PREP = 192;
 
 struct Scalars {  // per tensor, written by prepare_k
@@ -90,7 +90,7 @@ template <typename Row, int MAX> struct Args {
 using NormArgs = Args<TG, MAX_NORM>;
 static_assert(sizeof(Args<T32, MAX_T32>) < 4000, "kernel argument limit");
 static_assert(sizeof(Args<T8, MAX_T8>) < 4000, "kernel argument limit");
-static_assert(sizeof(NormArgs) < 4080, "kernel argument limit");
+static_assert(sizeof(NormArgs) + sizeof(DdlNormFold) < 4080, "kernel argument limit");
 
 struct PrepArgs {
   float* step[MAX_PREP];
@@ -135,25 +135,28 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 // norm = sqrt(sum of the partial sums) * mul; the coefficient that brings it
-// to max_norm.  NaN stays NaN, as in torch's clip_grad_norm_.
-__device__ __forceinline__ void fold_norm(const DdlNormFold& f) {
+// to max_norm, which one thread stores.  NaN stays NaN, as in torch's
+// clip_grad_norm_.
+__device__ __forceinline__ float fold_norm(const DdlNormFold& f, bool store) {
   double sum = 0.0;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < f.blocks; i += blockDim.x)
     sum += f.partials[i];
   sum = block_sum(sum);
-  if (threadIdx.x == 0) {
-    const float n = (float)(sqrt(sum) * f.mul);
+  const float n = (float)(sqrt(sum) * f.mul);
+  float k = (float)f.max_norm / (n + 1e-6f);
+  k = k >= 1.f ? 1.f : k;
+  if (store && threadIdx.x == 0) {
     *f.norm = n;
-    const float k = (float)f.max_norm / (n + 1e-6f);
-    *f.coef = k >= 1.f ? 1.f : k;
+    *f.coef = k;
   }
+  return k;
 }
 
 constexpr int FOLD_THREADS = 1024;
 
 __global__ __launch_bounds__(FOLD_THREADS) void fold_norm_k(DdlNormFold f) {
-  fold_norm(f);
+  fold_norm(f, true);
 }
 
 // One thread a tensor; the fold of the norm rides along.  beta^t is
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(FOLD_THREADS) void fold_norm_k(DdlNormFold f) {
 __global__ __launch_bounds__(FOLD_THREADS) void prepare_k(
     PrepArgs a, double lr, double log_beta1, double log_beta2, uint32_t seed,
     Scalars* out, DdlNormFold f) {
-  if (f.partials) fold_norm(f);
+  if (f.partials) fold_norm(f, true);
   const int i = threadIdx.x;
   if (i >= a.count) return;
   const float t = *a.step[i] + 1.f;
@@ -424,10 +427,11 @@ __global__ __launch_bounds__(THREADS) void grad_norm_k(NormArgs a,
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void grad_scale_k(
-    NormArgs a, const float* __restrict__ coef) {
-  const float k = *coef;
+// FOLD: the coefficient comes from the partial sums, which every block adds up.
+template <typename T, bool FOLD>
+__global__ __launch_bounds__(THREADS) void grad_scale_k(NormArgs a,
+                                                        DdlNormFold f) {
+  const float k = FOLD ? fold_norm(f, blockIdx.x == 0) : *f.coef;
   if (k == 1.f) return;
   const int ti = find_tensor(a.first, a.count, blockIdx.x);
   T* g = (T*)a.t[ti].g;
@@ -615,13 +619,19 @@ void ddl_grad_norm_fold(const DdlNormFold* f, hipStream_t s) {
 }
 
 void ddl_grad_scale(const DdlGradTensor* t, int64_t count, int dtype,
-                    const float* coef, hipStream_t s) {
+                    const DdlNormFold* f, int fold, hipStream_t s) {
   norm_groups(t, count, [&](const NormArgs& a, int blocks, int64_t) {
+#define RUN(T)                                                \
+  if (fold)                                                   \
+    grad_scale_k<T, true><<<blocks, THREADS, 0, s>>>(a, *f);  \
+  else                                                        \
+    grad_scale_k<T, false><<<blocks, THREADS, 0, s>>>(a, *f)
     switch (dtype) {
-      case 0: grad_scale_k<float><<<blocks, THREADS, 0, s>>>(a, coef); break;
-      case 1: grad_scale_k<bf16><<<blocks, THREADS, 0, s>>>(a, coef); break;
-      case 2: grad_scale_k<f16><<<blocks, THREADS, 0, s>>>(a, coef); break;
+      case 0: RUN(float); break;
+      case 1: RUN(bf16); break;
+      case 2: RUN(f16); break;
     }
+#undef RUN
   });
 }
 

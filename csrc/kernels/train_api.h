@@ -65,8 +65,14 @@ int64_t ddl_grad_norm_blocks(const DdlGradTensor* t, int64_t count);
 void ddl_grad_norm_partials(const DdlGradTensor* t, int64_t count, int dtype,
                             double* partials, hipStream_t s);
 void ddl_grad_norm_fold(const DdlNormFold* f, hipStream_t s);
-// g *= *coef; nothing is read or written where *coef is 1.
+// g *= coef, which is read from f->coef, or with `fold` made from the partial
+// sums on the way (ddl_grad_norm_fold is not needed then); nothing is read or
+// written where it is 1.
 void ddl_grad_scale(const DdlGradTensor* t, int64_t count, int dtype,
-                    const float* coef, hipStream_t s);
+                    const DdlNormFold* f, int fold, hipStream_t s);
+// Partial sums up to which the fold is better off in the scaling launch, whose
+// blocks each add up all of them: clipping 4 million elements (1956 sums) takes
+// 13 us so and 16 with a launch for the fold, 8 million (3908) 17 and 16.
+#define DDL_FOLD_IN_SCALE 2048
 
 }  // extern "C"

@@ -633,3 +633,35 @@ def test_tensors_that_share_memory_are_refused():
         clip_grad_norm_([a, c], 1.0)
     c.grad = base[50:]
     clip_grad_norm_([a, c], 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("n", [1 << 22, (1 << 22) + 1, 9_000_003])
+@pytest.mark.parametrize("captured", [False, True])
+def test_clip_of_many_elements(n, captured):
+    """Sizes about where the fold of the norm moves to a launch of its own."""
+    params = [make([n], torch.bfloat16, "cuda")[0],
+              make([1001], torch.float32, "cuda")[0]]
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = clip_grad_norm_(params, 2.0)
+    for scale in (0.25, 0.0001, 3.0):
+        grads = [torch.randn_like(p) * scale for p in params]
+        for p, g in zip(params, grads):
+            p.grad.copy_(g)
+        if captured:
+            graph.replay()
+        else:
+            norm = clip_grad_norm_(params, 2.0)
+        want = math.sqrt(sum(float(g.double().square().sum())
+                             for g in grads))
+        assert abs(float(norm) - want) <= 2 * U * want
+        coef = min(1.0, 2.0 / (want + 1e-6))
+        for p, g in zip(params, grads):
+            ref = g.double() * coef
+            half_step = torch.finfo(p.dtype).eps / 2
+            assert ((p.grad.double() - ref).abs()
+                    <= ref.abs() * (half_step + 6 * U)).all()
+            if coef == 1.0:
+                assert torch.equal(p.grad, g)
