@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void act_bwd_k(
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (act) activate_grad8(v[t], q[t], act);
+      if (act) activate_grad8<sizeof(T) == 2>(v[t], q[t], act);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         // a gradient of NaN behind the row's end would enter the products
