@@ -42,6 +42,12 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
+// What a kernel wrote: autograd's saved tensors are told, as of torch's own
+// updates.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void check_grad(const at::Tensor& g) {
   TORCH_CHECK(g.layout() == at::kStrided,
               "sparse gradients are not supported");
@@ -111,8 +117,7 @@ class AdamWPlan {
   // plan) of parameters with a gradient and no state.
   std::vector<int64_t> collect() {
     c10::DeviceGuard guard(device_);
-    rows_.clear();
-    grads_.clear();
+    forget();
     std::vector<int64_t> missing;
     for (const int64_t i : order_) {
       const at::Tensor& p = params_[i];
@@ -131,6 +136,7 @@ class AdamWPlan {
                   "the gradient of parameter ", indices_[i],
                   " differs from it in device or dtype");
       if (!same_layout(p, g)) {
+        at::NoGradGuard no_grad;
         at::Tensor copy = at::empty_like(p);
         copy.copy_(g);
         g = copy;
@@ -148,6 +154,7 @@ class AdamWPlan {
       r.step = s.step.data_ptr<float>();
       r.index = (uint32_t)indices_[i];
       rows_.push_back(r);
+      places_.push_back(i);
       grads_.push_back(std::move(g));
     }
     return missing;
@@ -177,8 +184,8 @@ class AdamWPlan {
       ddl_grad_norm_fold(fold, s);
     }
     C10_HIP_KERNEL_LAUNCH_CHECK();
-    rows_.clear();
-    grads_.clear();
+    for (const int64_t i : places_) written(params_[i]);
+    forget();
   }
 
   c10::Device device() const { return device_; }
@@ -188,6 +195,12 @@ class AdamWPlan {
   struct State {
     at::Tensor master, m, v, ms, vs, step;
   };
+
+  void forget() {
+    rows_.clear();
+    places_.clear();
+    grads_.clear();
+  }
 
   at::Tensor checked(const at::Tensor& t, at::ScalarType kind,
                      const char* name) const {
@@ -219,6 +232,7 @@ class AdamWPlan {
   at::ScalarType dtype_;
   std::vector<State> states_;
   std::vector<int64_t> order_;  // places, the largest parameter first
+  std::vector<int64_t> places_;  // of what collect() saw, as are these
   std::vector<DdlAdamTensor> rows_;
   Tensors grads_;
 };
@@ -231,7 +245,7 @@ struct NormList {
 // Partial sums of these lists, and where norm and coefficient go (0-dim
 // float32 tensors); the fold is still to be launched.
 struct Norm {
-  at::Tensor partials, norm, coef;
+  at::Tensor partials, norm;  // the coefficient lies behind the partial sums
   DdlNormFold fold;
 };
 
@@ -244,9 +258,8 @@ Norm norm_of(const std::vector<NormList>& lists, c10::Device device,
   for (const auto& l : lists)
     blocks += ddl_grad_norm_blocks(l.rows.data(), (int64_t)l.rows.size());
   out.partials =
-      at::empty({std::max<int64_t>(blocks, 1)}, opts.dtype(at::kDouble));
+      at::empty({blocks + 1}, opts.dtype(at::kDouble));
   out.norm = at::empty({}, opts.dtype(at::kFloat));
-  out.coef = at::empty({}, opts.dtype(at::kFloat));
   double* at = out.partials.data_ptr<double>();
   for (const auto& l : lists) {
     const int64_t n = (int64_t)l.rows.size();
@@ -255,7 +268,8 @@ Norm norm_of(const std::vector<NormList>& lists, c10::Device device,
   }
   out.fold = DdlNormFold{out.partials.data_ptr<double>(), blocks, mul,
                          max_norm, out.norm.data_ptr<float>(),
-                         out.coef.data_ptr<float>()};
+                         reinterpret_cast<float*>(
+                             out.partials.data_ptr<double>() + blocks)};
   return out;
 }
 
@@ -310,6 +324,7 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     const int dtype = code_of(g.scalar_type());
     if (g.numel() == 0) continue;
     lists[dtype].rows.push_back(DdlGradTensor{g.data_ptr(), g.numel()});
+    written(g);
     const char* start = static_cast<const char*>(g.const_data_ptr());
     places.emplace_back(start, start + g.nbytes());
   }

@@ -15,6 +15,8 @@ and biases) as required by the batch-8k config (BASELINE.json:9).
 from __future__ import annotations
 
 import torch
+from torch.optim.optimizer import (_global_optimizer_post_hooks,
+                                   _global_optimizer_pre_hooks)
 
 from ._ext import load_kernels_ext
 
@@ -462,17 +464,35 @@ class FusedAdamW(torch.optim.Optimizer):
 
     # ---- step -------------------------------------------------------------
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # The base class would wrap this for hooks and profiles, 6 us of the
+        # host a step, where the kernels of a small model take as long.
+        if (closure is not None or _global_optimizer_pre_hooks
+                or _global_optimizer_post_hooks
+                or self._optimizer_step_pre_hooks
+                or self._optimizer_step_post_hooks
+                or torch.autograd._profiler_enabled()):
+            return self._hooked_step(closure)
+        self._update()
+
+    step.hooked = True
+
+    def _closure_step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if any(p.is_cuda for g in self.param_groups for p in g["params"]):
+        self._update()
+        return loss
+
+    _hooked_step = torch.optim.Optimizer.profile_hook_step(_closure_step)
+
+    def _update(self):
+        if self._plans is not None or any(
+                p.is_cuda for g in self.param_groups for p in g["params"]):
             self._step_gpu()
         else:
             self._step_cpu()
-        return loss
 
     def _check_overlap(self):
         """Tensors of one launch are updated at the same time."""
@@ -520,8 +540,9 @@ class FusedAdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("take a step before capturing one: a "
                                    "replay would begin with new states")
-            for i, members, bits in missing:
-                self._init_state(members[i], bits)
+            with torch.no_grad():
+                for i, members, bits in missing:
+                    self._init_state(members[i], bits)
             self._build_plans()
             for plan, _, _ in self._plans:
                 plan.collect()
@@ -533,6 +554,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if norm is not None:
             self.grad_norm = norm
 
+    @torch.no_grad()
     def _step_cpu(self):
         mul = 1.0 / self.grad_scale
         if self.max_grad_norm is not None:
@@ -604,7 +626,6 @@ def _norm_cpu(grads, mul, max_norm):
     return norm, (max_norm / (norm + 1e-6)).clamp(max=1.0)
 
 
-@torch.no_grad()
 def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
     """Scale all gradients in place so that their global 2-norm is at most
     ``max_norm``; returns the norm before (0-dim float32, no host sync).
@@ -633,6 +654,7 @@ def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
     grads = [p.grad for p in params if p.grad is not None]
     norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
     if not float(coef) == 1.0:
-        for g in grads:
-            g.copy_(g.float() * coef)
+        with torch.no_grad():
+            for g in grads:
+                g.copy_(g.float() * coef)
     return norm

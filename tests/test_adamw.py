@@ -13,6 +13,7 @@ import math
 
 import pytest
 import torch
+from torch.optim.optimizer import register_optimizer_step_pre_hook
 
 from distributeddeeplearning_amd.ops import FusedAdamW, clip_grad_norm_
 from distributeddeeplearning_amd.ops import optim as O
@@ -665,3 +666,54 @@ def test_clip_of_many_elements(n, captured):
                     <= ref.abs() * (half_step + 6 * U)).all()
             if coef == 1.0:
                 assert torch.equal(p.grad, g)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_hooks_closures_and_profiles(device):
+    p = make([20], torch.float32, device)[0]
+    opt = FusedAdamW([p])
+    calls = []
+    handles = [
+        opt.register_step_pre_hook(lambda *a: calls.append("pre")),
+        opt.register_step_post_hook(lambda *a: calls.append("post")),
+        register_optimizer_step_pre_hook(lambda *a: calls.append("all"))]
+    assert opt.step() is None
+    assert calls == ["all", "pre", "post"]
+    for h in handles:
+        h.remove()
+    opt.step()
+    assert len(calls) == 3
+
+    def closure():
+        assert torch.is_grad_enabled()
+        opt.zero_grad()
+        loss = (p * p).sum()
+        loss.backward()
+        return loss
+
+    before = float(p.detach().square().sum())
+    assert abs(float(opt.step(closure)) - before) <= 32 * U * before
+    with torch.profiler.profile(
+            activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any("FusedAdamW.step" in e.key for e in prof.key_averages())
+    assert float(opt.state[p]["step"]) == 4
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    opt.step()
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 5e-4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autograd_sees_that_values_changed(device):
+    p = make([20], torch.float32, device)[0]
+    opt = FusedAdamW([p])
+    loss = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    x = torch.ones(20, device=device, requires_grad=True)
+    loss = (x * p.grad).sum()
+    clip_grad_norm_([p], 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
