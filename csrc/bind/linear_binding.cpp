@@ -1,5 +1,5 @@
 // Torch binding of the dense layer (csrc/kernels/linear*.hip): checks, packs
-// operands whose rows do not lie on 16-byte boundaries, allocates outputs and
+// operands whose rows do not begin at 4 bytes, allocates outputs and
 // workspaces, and launches on the current stream of the tensors' device.  The
 // autograd function is here too: in Python it would cost a small layer more
 // time than its kernels.
@@ -48,17 +48,20 @@ int64_t row_stride(const at::Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
-// Rows that the tiled kernel reads as they are: they begin and end at 16
-// bytes, and are no further apart than its 32-bit offsets inside a tile reach.
+// Rows that the tiled kernel reads as they are: they begin at 4 bytes, and are
+// no further apart than its 32-bit offsets inside a tile reach.
 int64_t reach(const at::Tensor& t) {
   return ((int64_t)1 << 31) / 256 / t.element_size();
 }
 
+bool begins_at(const at::Tensor& t, int64_t bytes) {
+  return (t.size(1) <= 1 || t.stride(1) == 1) &&
+         (t.size(0) <= 1 || t.stride(0) * t.element_size() % bytes == 0) &&
+         (uintptr_t)t.const_data_ptr() % bytes == 0;
+}
+
 bool fits(const at::Tensor& t) {
-  const int64_t per = 16 / t.element_size();
-  return (t.size(1) <= 1 || t.stride(1) == 1) && row_stride(t) % per == 0 &&
-         t.size(1) % per == 0 && row_stride(t) < reach(t) &&
-         ((uintptr_t)t.const_data_ptr() & 15) == 0;
+  return begins_at(t, 4) && row_stride(t) < reach(t);
 }
 
 // The same matrices with rows padded by zeros to 16 bytes where they do not
@@ -126,7 +129,9 @@ at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
   }
   if (m == 0 || n == 0) return y;
   const int64_t floats = ddl_product_plan(&p);
-  const bool few = ddl_few_rows_pay(&p, fits(x) && fits(w));
+  const bool few =
+      ddl_few_rows_pay(&p, begins_at(x, 16) && begins_at(w, 16),
+                       !fits(x) || !fits(w));
   if (few) {
     x = inner_contiguous(x);
     w = inner_contiguous(w);

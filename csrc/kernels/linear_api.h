@@ -9,9 +9,8 @@ extern "C" {
 
 // out[i][j] = epilogue(sum_r a(i, r) b(j, r)).  An operand is stored with r
 // contiguous (`*_col` 0: a(i, r) = a[i * lda + r]) or with the output's index
-// contiguous (`*_col` 1: a(i, r) = a[r * lda + i]).  What is contiguous is a
-// multiple of 16 bytes long (zeros behind the end of r), rows begin at
-// 16-byte boundaries.
+// contiguous (`*_col` 1: a(i, r) = a[r * lda + i]).  Rows begin at 4 bytes and
+// end anywhere; what lies between them does not count.
 struct DdlProduct {
   const void* a;
   const void* b;
@@ -40,9 +39,9 @@ void ddl_product(const DdlProduct* p, hipStream_t s);
 
 // The same for at most 16 rows, both operands with r contiguous and rows
 // anywhere (any lda, ldb, r and alignment); needs no slabs.  Whether that is
-// estimated to be faster than the planned product; `aligned`: its operands
-// would not have to be packed.
-bool ddl_few_rows_pay(const DdlProduct* p, bool aligned);
+// estimated to be faster than the planned product; `aligned`: all rows begin at
+// 16 bytes, `packed`: the planned one's operands would have to be packed.
+bool ddl_few_rows_pay(const DdlProduct* p, bool aligned, bool packed);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
 // dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of

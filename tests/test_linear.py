@@ -256,6 +256,23 @@ def test_what_lies_beyond_is_not_read(device):
         run_case(*shape, torch.bfloat16, device, "gelu", change=change)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 6, 7, 9, 10, 12, 14, 30, 31, 33,
+                               34, 62, 63, 65, 66, 70, 127, 130, 1029, 4098])
+def test_rows_that_end_inside_a_load(k, dtype):
+    """NaN between the rows, which begin at 4 bytes (odd ones at 2)."""
+    def change(t):
+        if t.dim() == 1:
+            return t.detach()
+        gap = 2 if t.shape[1] % 2 == 0 else 3
+        wide = torch.full((t.shape[0], t.shape[1] + gap), float("nan"),
+                          dtype=t.dtype, device=t.device)
+        return wide[:, gap - 1 & ~1:][:, :t.shape[1]].copy_(t).detach()
+    run_case(67, k, 46, dtype, "cuda", "none", change=change)
+    run_case(300, 38, k, dtype, "cuda", "gelu", change=change)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("m,k,n", [(0, 4, 5), (3, 0, 5), (3, 4, 0)])
 def test_empty(m, k, n, device):
