@@ -54,14 +54,10 @@ int64_t reach(const at::Tensor& t) {
   return ((int64_t)1 << 31) / 256 / t.element_size();
 }
 
-bool begins_at(const at::Tensor& t, int64_t bytes) {
-  return (t.size(1) <= 1 || t.stride(1) == 1) &&
-         (t.size(0) <= 1 || t.stride(0) * t.element_size() % bytes == 0) &&
-         (uintptr_t)t.const_data_ptr() % bytes == 0;
-}
-
 bool fits(const at::Tensor& t) {
-  return begins_at(t, 4) && row_stride(t) < reach(t);
+  return (t.size(1) <= 1 || t.stride(1) == 1) &&
+         (t.size(0) <= 1 || t.stride(0) * t.element_size() % 4 == 0) &&
+         row_stride(t) < reach(t) && ((uintptr_t)t.const_data_ptr() & 3) == 0;
 }
 
 // The same matrices with rows padded by zeros to 16 bytes where they do not
@@ -129,9 +125,7 @@ at::Tensor forward_of(at::Tensor& x, at::Tensor& w, const Maybe& bias,
   }
   if (m == 0 || n == 0) return y;
   const int64_t floats = ddl_product_plan(&p);
-  const bool few =
-      ddl_few_rows_pay(&p, begins_at(x, 16) && begins_at(w, 16),
-                       !fits(x) || !fits(w));
+  const bool few = ddl_few_rows_pay(&p, fits(x) && fits(w));
   if (few) {
     x = inner_contiguous(x);
     w = inner_contiguous(w);

@@ -284,16 +284,17 @@ void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
 // block of the former reads its part of W at 28 KB a us, less with more rows
 // of x beside it, and a third of that where 2-byte rows begin anywhere: 16 x
 // 25088 -> 4096 takes 46 us (tiled 34), 1 x 16384 -> 128 20 (10), 16 x 4096 ->
-// 4096 10.9 (12.5), 1 x 2047 -> 1001 10.7 (13.6, of which packing 5).
-bool ddl_few_rows_pay(const DdlProduct* p, bool aligned, bool packed) {
+// 4096 10.9 (12.5), 1 x 2047 -> 1001 10.7 (13.6, of which packing 5), 1 x 4098
+// -> 4096 8.1 (11.8); float32, 16 x 14242 -> 2853 45 (71).
+bool ddl_few_rows_pay(const DdlProduct* p, bool aligned) {
   if (p->m > 16 || p->n >= ((int64_t)1 << 26)) return false;  // its grid
   const float size = p->dtype == 0 ? 4.f : 2.f;
   const float row = p->r * size, all = row * p->n;
-  float rate = 28e3f / (1.f + 0.8f * p->m / 16.f);
+  float rate = 28e3f / (1.f + (p->dtype == 0 ? 0.4f : 0.8f) * p->m / 16.f);
   if (!aligned && p->dtype != 0) rate /= 3.f;
   const float rounds = std::ceil(p->n / (16.f * compute_units()));
   const float few = 1.f + std::max(all / 5.5e6f, rounds * 16.f * row / rate);
-  const float tiled = p->us + (packed ? 5.f + all / 2e6f : 0.f);
+  const float tiled = p->us + (aligned ? 0.f : 5.f + all / 2e6f);
   return few <= tiled;
 }
 

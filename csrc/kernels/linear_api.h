@@ -39,9 +39,9 @@ void ddl_product(const DdlProduct* p, hipStream_t s);
 
 // The same for at most 16 rows, both operands with r contiguous and rows
 // anywhere (any lda, ldb, r and alignment); needs no slabs.  Whether that is
-// estimated to be faster than the planned product; `aligned`: all rows begin at
-// 16 bytes, `packed`: the planned one's operands would have to be packed.
-bool ddl_few_rows_pay(const DdlProduct* p, bool aligned, bool packed);
+// estimated to be faster than the planned product; `aligned`: its operands
+// would not have to be packed.
+bool ddl_few_rows_pay(const DdlProduct* p, bool aligned);
 void ddl_product_few(const DdlProduct* p, hipStream_t s);
 
 // dz[i][j] = dy[i][j] act'(z[i][j]), zeros in columns n..lddz (a multiple of
