@@ -179,24 +179,41 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
       dz = at::empty({m, round_up(n, 8)}, x.options());
     }
   }
+  DdlProduct px{}, pw{};
+  int64_t fx = 0, fw = 0;
+  bool small = false;
+  if (products) {
+    px.dtype = dtype;
+    px.b_col = 1;
+    px.n = k;
+    px.ldo = k;
+    pw = px;
+    pw.a_col = 1;
+    px.m = pw.r = m;
+    px.r = pw.m = n;
+    if (want_dx) fx = ddl_product_plan(&px);
+    if (want_dw) fw = ddl_product_plan(&pw);
+    small = want_dx && want_dw && ddl_small_backward(&px, &pw);
+  }
   DdlBiasFold fold{};
   at::Tensor partials;
   if (want_db) {
-    fold.chunks = ddl_bias_chunks(m, n);
     fold.n = n;
-    partials = at::empty({fold.chunks * n}, x.options().dtype(at::kFloat));
-    fold.partials = partials.data_ptr<float>();
     fold.dbias = out.db.data_ptr();
+    if (act || !small) {
+      fold.chunks = ddl_bias_chunks(m, n);
+      partials = at::empty({fold.chunks * n}, x.options().dtype(at::kFloat));
+      fold.partials = partials.data_ptr<float>();
+    }
   }
-  if (want_db || dz.defined())
+  if (fold.partials || dz.defined())
     ddl_act_bwd(d.const_data_ptr(), row_stride(d),
                 act ? zc.const_data_ptr() : nullptr,
                 act && zc.scalar_type() == at::kFloat,
                 act ? row_stride(zc) : 0,
                 dz.defined() ? dz.data_ptr() : nullptr,
                 dz.defined() ? dz.size(1) : 0, m, n, (int)act, dtype,
-                want_db ? partials.data_ptr<float>() : nullptr, s);
-  DdlProduct px{}, pw{};
+                fold.partials ? partials.data_ptr<float>() : nullptr, s);
   if (products) {
     if (!act) {
       dz = d;
@@ -205,27 +222,15 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
     } else {
       pack(want_dx ? &w : nullptr, want_dw ? &x : nullptr);
     }
-    px.dtype = dtype;
-    px.a = dz.const_data_ptr();
-    px.lda = row_stride(dz);
-    px.b_col = 1;
-    px.n = k;
-    px.ldo = k;
-    pw = px;
+    px.a = pw.a = dz.const_data_ptr();
+    px.lda = pw.lda = row_stride(dz);
     px.b = w.const_data_ptr();
     px.ldb = row_stride(w);
-    px.m = m;
-    px.r = n;
     pw.b = x.const_data_ptr();
     pw.ldb = row_stride(x);
-    pw.a_col = 1;
-    pw.m = n;
-    pw.r = m;
     if (want_dx) px.out = out.dx.data_ptr();
     if (want_dw) pw.out = out.dw.data_ptr();
-    const int64_t fx = want_dx ? ddl_product_plan(&px) : 0;
-    const int64_t fw = want_dw ? ddl_product_plan(&pw) : 0;
-    if (want_dx && want_dw && ddl_small_backward(&px, &pw)) {
+    if (small) {
       ddl_backward_small(&px, &pw, &fold, s);
       fold.n = 0;
     } else {

@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void act_bwd_k(
 template <typename T>
 __global__ __launch_bounds__(256) void fold_bias_k(DdlBiasFold f) {
   __shared__ __align__(16) char smem[256 * sizeof(double)];
-  fold_bias<T>(f, blockIdx.x, smem);
+  fold_bias(f.partials, f.n, f.chunks, (T*)f.dbias, f.n, blockIdx.x, smem);
 }
 
 // ---- rows that do not begin at 4 bytes --------------------------------------

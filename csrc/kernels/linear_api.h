@@ -62,7 +62,9 @@ struct DdlBiasFold {
 void ddl_fold_bias(const DdlBiasFold* f, int dtype, hipStream_t s);
 
 // dx and dw, planned, and the fold in one launch, where that is estimated to
-// be faster than a launch each.
+// be faster than a launch each.  Without partials the bias gradient is summed
+// from dw's a: 64 x 64 -> 96 bf16 takes 8.4 us so, 11.0 with partial sums made
+// first, 2048 x 64 -> 64 18.8 (21.3).
 bool ddl_small_backward(const DdlProduct* dx, const DdlProduct* dw);
 void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
                         const DdlBiasFold* bias, hipStream_t s);

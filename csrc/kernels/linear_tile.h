@@ -638,26 +638,28 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_k(Product p) {
       p, xcd_swizzle(blockIdx.x, gridDim.x), smem);
 }
 
-// The fold of act_bwd_k's partial sums: FOLD_COLS columns a block of 256.
+// The bias gradient from partial sums of act_bwd_k (T: float), or from dz
+// itself where the small backward pass has it anyway: FOLD_COLS columns a block
+// of 256 threads.
 constexpr int FOLD_COLS = 16;
 
-template <typename T>
-__device__ __forceinline__ void fold_bias(const DdlBiasFold& f, int64_t block,
-                                          char* smem) {
+template <typename From, typename T>
+__device__ __forceinline__ void fold_bias(const From* rows, int64_t ld,
+                                          int64_t count, T* dbias, int64_t n,
+                                          int64_t block, char* smem) {
   constexpr int LANES = 256 / FOLD_COLS;
   double* part = reinterpret_cast<double*>(smem);
   const int col = threadIdx.x % FOLD_COLS, lane = threadIdx.x / FOLD_COLS;
   const int64_t j = block * FOLD_COLS + col;
   double sum = 0.0;
-  if (j < f.n)
+  if (j < n)
 #pragma unroll 8
-    for (int64_t c = lane; c < f.chunks; c += LANES)
-      sum += f.partials[c * f.n + j];
+    for (int64_t c = lane; c < count; c += LANES) sum += to_f32(rows[c * ld + j]);
   part[threadIdx.x] = sum;
   __syncthreads();
-  if (lane == 0 && j < f.n) {
+  if (lane == 0 && j < n) {
     for (int k = 1; k < LANES; ++k) sum += part[k * FOLD_COLS + col];
-    ((T*)f.dbias)[j] = from_f32<T>((float)sum);
+    dbias[j] = from_f32<T>((float)sum);
   }
 }
 
@@ -675,7 +677,13 @@ __global__ __launch_bounds__(256, 2) void backward_small_k(
   } else if (id < nx + nw) {
     product_block<T, 64, 64, 4, 1, 4, true, true>(dw, id - nx, smem);
   } else {
-    fold_bias<T>(bias, id - nx - nw, smem);
+    id -= nx + nw;
+    if (bias.partials)
+      fold_bias(bias.partials, bias.n, bias.chunks, (T*)bias.dbias, bias.n, id,
+                smem);
+    else
+      fold_bias((const T*)dw.a, dw.lda / (int64_t)sizeof(T), dw.r,
+                (T*)bias.dbias, bias.n, id, smem);
   }
 }
 
