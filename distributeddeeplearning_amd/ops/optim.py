@@ -460,7 +460,9 @@ class FusedAdamW(torch.optim.Optimizer):
         return state
 
     def invalidate_table(self):
-        """Nothing to do: gradients are looked up at every step."""
+        """Looks the parameters up anew at the next step, after some were
+        replaced in ``param_groups``.  Gradients always are."""
+        self._plans = None
 
     # ---- step -------------------------------------------------------------
 
@@ -652,6 +654,8 @@ def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
         return load_kernels_ext().clip_grads(params, 1.0 / grad_scale,
                                              float(max_norm))
     grads = [p.grad for p in params if p.grad is not None]
+    if len({id(g) for g in grads}) != len(grads):
+        raise RuntimeError("a gradient appears twice")
     norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
     if not float(coef) == 1.0:
         with torch.no_grad():

@@ -717,3 +717,17 @@ def test_autograd_sees_that_values_changed(device):
     clip_grad_norm_([p], 1e-3)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_replaced_parameter_and_gradient_given_twice(device):
+    a, b = make([30, 30], torch.float32, device)
+    opt = FusedAdamW([a])
+    opt.step()
+    opt.param_groups[0]["params"][0] = b
+    opt.invalidate_table()
+    before, kept = b.detach().clone(), a.detach().clone()
+    opt.step()
+    assert torch.equal(a, kept) and not torch.equal(b, before)
+    with pytest.raises(RuntimeError, match="twice"):
+        clip_grad_norm_([a, b, a], 1.0)
