@@ -577,3 +577,21 @@ def test_tensors_that_are_not_what_lies_in_memory_are_refused():
         with pytest.raises(NotImplementedError, match="weight"):
             DF.linear_act(x, dual)
         assert DF.linear_act(x, w).shape == (3, 5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(5, 24, 40), (130, 70, 66), (600, 520, 1030)])
+@pytest.mark.parametrize("how", ["all", "rows", "columns"])
+def test_gradients_that_repeat_in_memory(shape, dtype, how):
+    """dy expanded from one number, one row or one column: as its copy."""
+    m, k, n = shape
+    torch.manual_seed(0)
+    leaves = [torch.randn(s, device="cuda").to(dtype).requires_grad_(True)
+              for s in ((m, k), (n, k), (n,))]
+    one = {"all": (1, 1), "rows": (1, n), "columns": (m, 1)}[how]
+    dy = torch.randn(one, device="cuda").to(dtype).expand(m, n)
+    y = DF.linear_act(*leaves)
+    got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    want = torch.autograd.grad(y, leaves, dy.contiguous())
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
