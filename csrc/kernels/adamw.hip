@@ -20,7 +20,11 @@
 // would never move.  So a code is rounded up with the probability of the part
 // that rounding down drops, by 16 bits of a hash of (seed, step, tensor,
 // element): the expected code is the value, and a run can be repeated bit
-// for bit.
+// for bit.  One exception: a positive r takes at least the smallest code,
+// 2^-9 of a scale.  Rounded to zero, r would leave the next step without its
+// denominator while m, drawn by other bits, may have been rounded up: with
+// gradients at 1e-6 of their block's largest, steps of the first twenty reached
+// 364 times lr; they reach 1.5 times so (float32 moments: 1.0).
 //
 // This file is compiled without fast-math: infinities and NaN keep their
 // meaning, divisions and roots are correctly rounded.  Products and sums of
@@ -272,6 +276,8 @@ __device__ __forceinline__ float half_wave_max(float x) {
 // Codes of 8 values of a lane, whose block's largest finite magnitude is
 // `top`.  An infinite or NaN value becomes a NaN code and leaves its block's
 // scale alone; a block whose values are all below 2^-100 becomes zeros.
+// LEAST: a positive value of another block takes at least the smallest code.
+template <bool LEAST>
 __device__ __forceinline__ uint2 encode8(const float* x, float top,
                                          const uint32_t* r, int shift,
                                          float& scale) {
@@ -282,8 +288,9 @@ __device__ __forceinline__ uint2 encode8(const float* x, float top,
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float y = fminf(fabsf(x[j]) * inv, 448.f);
-    const float e = copysignf(
-        round_by_chance(y, (r[j] >> shift) & 0xFFFFu), x[j]);
+    float code = round_by_chance(y, (r[j] >> shift) & 0xFFFFu);
+    if (LEAST && y > 0.f) code = fmaxf(code, 0x1p-9f);
+    const float e = copysignf(code, x[j]);
     q[j] = finite(x[j]) ? e : __uint_as_float(0x7FC00000u);
   }
   return uint2{pack4(q), pack4(q + 4)};
@@ -356,8 +363,8 @@ __global__ __launch_bounds__(THREADS) void adamw8_k(
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = mix((uint32_t)(i + j) ^ s.key);
     float ms_new, vs_new;
-    const uint2 mq = encode8(m, mtop, r, 0, ms_new);
-    const uint2 vq = encode8(root, vtop, r, 16, vs_new);
+    const uint2 mq = encode8<false>(m, mtop, r, 0, ms_new);
+    const uint2 vq = encode8<true>(root, vtop, r, 16, vs_new);
     if (lane == 0) {
       t.ms[block] = ms_new;
       t.vs[block] = vs_new;

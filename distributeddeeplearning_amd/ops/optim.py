@@ -256,12 +256,14 @@ def _blocks(x: torch.Tensor) -> torch.Tensor:
     return torch.nn.functional.pad(x, (0, pad)).view(-1, MOMENT_BLOCK)
 
 
-def quantize_moment(x: torch.Tensor, r16: torch.Tensor):
+def quantize_moment(x: torch.Tensor, r16: torch.Tensor, least: bool = False):
     """8-bit codes (uint8 bits of e4m3) and block scales of a flat float32
     tensor.  A magnitude between two codes takes the upper one where the part
     above the lower, in 2^-16 of their distance, plus ``r16`` (int64 in
     [0, 2^16)) reaches 2^16.  Values that are not finite become NaN codes and
-    do not enter their block's scale; a block below 2^-100 becomes zeros."""
+    do not enter their block's scale; a block below 2^-100 becomes zeros.
+    ``least``: magnitudes above zero take at least the smallest code, 2^-9
+    (of sqrt(v), whose zero would leave a step without its denominator)."""
     n = x.numel()
     finite = torch.isfinite(x)
     top = _blocks(torch.where(finite, x.abs(), 0.0)).amax(1)
@@ -274,6 +276,8 @@ def quantize_moment(x: torch.Tensor, r16: torch.Tensor):
     normal = bits.int().view(torch.float32)
     small = torch.floor(y * 512.0 + r16.float() * 2.0 ** -16) / 512.0
     q = torch.where(y < 2.0 ** -6, small, normal)
+    if least:
+        q = torch.where(y > 0, q.clamp(min=2.0 ** -9), q)
     q = torch.where(finite, torch.copysign(q, x), float("nan"))
     return q.to(torch.float8_e4m3fn).view(torch.uint8), scale
 
@@ -301,7 +305,9 @@ class FusedAdamW(torch.optim.Optimizer):
     consecutive elements: 2 bytes a parameter for both moments instead of 8.
     Codes are rounded up or down by chance, so that they are right on
     average; the chance is a hash of ``seed``, the step, the tensor and the
-    element, so that a run can be repeated bit for bit.
+    element, so that a run can be repeated bit for bit.  ``sqrt(v)`` below
+    1 / 229376 of the largest of its 256 is held as that: such an element's
+    steps are shorter than with float32 moments.
 
     ``max_grad_norm`` clips the global norm of all gradients of the optimizer
     (as ``clip_grad_norm_`` before the step would, without writing the
@@ -600,7 +606,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     for name, code, new, bits16 in (
                             ("exp_avg", codes[0], m_new, r & 0xFFFF),
                             ("exp_avg_sq", codes[1], root, r >> 16)):
-                        q, scale = quantize_moment(new, bits16)
+                        q, scale = quantize_moment(
+                            new, bits16, least=name == "exp_avg_sq")
                         code.copy_(q)
                         st[name + "_scale"].copy_(scale)
                 else:

@@ -731,3 +731,83 @@ def test_replaced_parameter_and_gradient_given_twice(device):
     assert torch.equal(a, kept) and not torch.equal(b, before)
     with pytest.raises(RuntimeError, match="twice"):
         clip_grad_norm_([a, b, a], 1.0)
+
+
+# ---- second moments far below their block's largest -------------------------
+
+def _spread(n, small):
+    """One element of size one a block, the others of size `small`."""
+    scale = torch.full((n,), small)
+    scale[::256] = 1.0
+    return scale
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("small", [1e-4, 1e-5, 1e-7])
+def test_8_bit_second_moment_above_zero_keeps_a_code(device, small):
+    """A zero in the place of a small sqrt(v) would leave the next step
+    without its denominator; a zero stays one where there was no gradient."""
+    scale = _spread(3000, small)
+    scale[7] = scale[300] = 0.0
+    p = torch.nn.Parameter(torch.zeros(3000, device=device))
+    opt = FusedAdamW([p], state_bits=8, seed=2)
+    gen = torch.Generator().manual_seed(0)
+    for _ in range(6):
+        g = torch.randn(3000, generator=gen) * scale
+        p.grad = g.to(device)
+        opt.step()
+        code = opt.state[p]["exp_avg_sq"].cpu()
+        assert torch.equal(code == 0, scale == 0)
+    _, v = opt.moments(p)
+    least = opt.state[p]["exp_avg_sq_scale"].cpu() * 2.0 ** -9
+    least = least.repeat_interleave(256)[:3000]
+    assert (v.cpu().sqrt() >= least * (1 - 4 * U))[scale > 0].all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_8_bit_steps_are_bounded_where_gradients_spread(device, dtype):
+    """Elements at 1e-7 of their block's largest: sqrt(v) lies below its
+    smallest code and takes it, b = rtop / 448 / 512.  Each rounding of m adds
+    at most one smallest code of m, a = mtop / 448 / 512, which fades by 0.9 a
+    step: m <= 9 a + 0.1 |g| after many.  mtop <= K rtop by Cauchy and Schwarz
+    with K = 0.1 / sqrt(0.001) / sqrt(1 - 0.81 / 0.999) = 7.27, and with an
+    eighth for the rounding of the largest codes.  So m / sqrt(v) is below
+    9 * 7.27 * 9 / 8 + 3.2, and 20 steps' corrections make a step of it:
+    sqrt(1 - 0.999^20) / (1 - 0.9^20) = 0.161 (less before): 12.4 lr.  The
+    largest elements hold float32's bound, 1.16 lr, but for an eighth a step
+    in m and in sqrt(v)."""
+    n, lr = 4096, 1e-3
+    scale = _spread(n, 1e-7)
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=device))
+    # float16 does not hold 1e-7 well: gradients are scaled up
+    opt = FusedAdamW([p], lr=lr, weight_decay=0.0, state_bits=8, seed=2,
+                     eps=1e-12, grad_scale=256.0)
+    gen = torch.Generator().manual_seed(0)
+    before = torch.zeros(n)
+    for _ in range(20):
+        g = torch.randn(n, generator=gen).clamp(-4, 4) * scale * 256.0
+        p.grad = g.to(device, dtype)
+        opt.step()
+        w = opt.state[p].get("master", p).detach().float().cpu().clone()
+        assert float((w - before).abs().max()) < 12.4 * lr
+        before = w
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0, 1])
+def test_8_bit_codes_of_spread_gradients_equal_the_cpu_path(dtype, offset):
+    scale = 10.0 ** (torch.arange(5000) % 9 - 8.0)
+    runs = []
+    for device in ("cpu", "cuda"):
+        p, = make([5000], dtype, device, offset=offset)
+        opt = FusedAdamW([p], lr=1e-2, state_bits=8, seed=5, grad_scale=64.0)
+        gen = torch.Generator().manual_seed(1)
+        for _ in range(3):
+            g = torch.randn(5000, generator=gen) * scale * 64.0
+            p.grad.copy_(g.to(device, dtype))
+            opt.step()
+        runs.append(state_of(opt, p))
+    for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+        assert torch.equal(runs[0][k], runs[1][k]), k
