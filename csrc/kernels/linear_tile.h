@@ -125,7 +125,6 @@ __device__ __forceinline__ float activate(float z, int act) {
 template <bool FAST>
 __device__ __forceinline__ float activate_grad(float z, int act) {
   switch (act) {
-    case 1: return z <= 0.f ? 0.f : 1.f;
     case 2: {
       float e;
       const float phi = normal<FAST>(z, e);
@@ -207,7 +206,8 @@ __device__ __forceinline__ void activate8(float* y, int act) {
   }
 }
 
-// v[k] *= act'(z[k])
+// v[k] *= act'(z[k]).  ReLU's is a choice, no product: what arrives where it
+// is shut is dropped, also an infinity or NaN.
 template <bool FAST>
 __device__ __forceinline__ void activate_grad8(float* v, const float* z,
                                                int act) {
@@ -216,7 +216,10 @@ __device__ __forceinline__ void activate_grad8(float* v, const float* z,
     for (int k = 0; k < 8; ++k) v[k] *= activate_grad<FAST>(z[k], which.value);
   };
   switch (act) {
-    case 1: all(std::integral_constant<int, 1>{}); break;
+    case 1:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = z[k] <= 0.f ? 0.f : v[k];
+      break;
     case 2: all(std::integral_constant<int, 2>{}); break;
     case 3: all(std::integral_constant<int, 3>{}); break;
     case 4: all(std::integral_constant<int, 4>{}); break;

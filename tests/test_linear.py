@@ -595,3 +595,39 @@ def test_gradients_that_repeat_in_memory(shape, dtype, how):
     got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
     want = torch.autograd.grad(y, leaves, dy.contiguous())
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(9, 24, 8), (40, 31, 50), (300, 40, 264)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_relu_stops_gradients_that_are_not_finite(shape, residual, dtype,
+                                                  device):
+    """Even outputs are negative: what arrives at them counts as zero,
+    infinite or not.  At a positive one it stays in its row and output."""
+    m, k, n = shape
+    gen = torch.Generator().manual_seed(0)
+    x = torch.rand(m, k, generator=gen) + 0.1
+    w = torch.rand(n, k, generator=gen) + 0.1
+    w[::2] *= -1
+    b = torch.zeros(n)
+    leaves = [t.to(device, dtype).requires_grad_(True) for t in (x, w, b)]
+    r = torch.zeros(m, n, device=device, dtype=dtype) if residual else None
+    dy = torch.randn(m, n, generator=gen).to(device, dtype)
+    dy[1, 0] = dy[2, 2] = dy[m - 1, 6] = 0.0
+
+    def grads():
+        return torch.autograd.grad(
+            DF.linear_act(*leaves, "relu", r), leaves, dy)
+
+    clean = grads()
+    dy[1, 0], dy[2, 2] = float("inf"), float("nan")
+    dy[m - 1, 6] = -float("inf")
+    assert all(torch.equal(p, q) for p, q in zip(clean, grads()))
+    dy[3, 1] = float("inf")
+    dx, dw, db = grads()
+    for got, ref, at in ((dx, clean[0], 3), (dw, clean[1], 1),
+                         (db, clean[2], 1)):
+        assert (got[at] == float("inf")).all()
+        keep = [i for i in range(len(ref)) if i != at]
+        assert torch.equal(got[keep], ref[keep])
