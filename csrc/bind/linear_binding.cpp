@@ -151,6 +151,7 @@ struct Grads {
 // z: what the activation took, in float32 (its output, in x's dtype, does for
 // ReLU); not looked at without an activation.  x and w may be padded copies of
 // matrices with k columns.
+// dy may be a lazy negation (autograd leaves them behind conjugates).
 Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
                   const at::Tensor& z, int64_t k, int64_t act, bool want_dx,
                   bool want_dw, bool want_db) {
@@ -169,7 +170,7 @@ Grads backward_of(const at::Tensor& dy, at::Tensor x, at::Tensor w,
   }
   if (m == 0 || n == 0) return out;
 
-  at::Tensor d = inner_contiguous(dy), dz, zc;
+  at::Tensor d = inner_contiguous(dy.resolve_neg()), dz, zc;
   const bool products = k > 0 && (want_dx || want_dw);
   if (act) {
     zc = inner_contiguous(z);

@@ -631,3 +631,31 @@ def test_relu_stops_gradients_that_are_not_finite(shape, residual, dtype,
         assert (got[at] == float("inf")).all()
         keep = [i for i in range(len(ref)) if i != at]
         assert torch.equal(got[keep], ref[keep])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_lazily_negated_gradient(act, device):
+    """As the imaginary part of a conjugate leaves it: its sign counts."""
+    torch.manual_seed(0)
+    x, w, b, r = (torch.randn(*s, device=device, requires_grad=True)
+                  for s in ((4, 8), (1, 8), (1,), (4, 1)))
+    leaves = (x, w, b, r)
+    c = torch.randn(4, 1, device=device, dtype=torch.complex64)
+    y = DF.linear_act(x, w, b, act, r)
+    seen = []
+    y.register_hook(lambda g: seen.append(g))
+    loss = (torch.complex(torch.zeros_like(y), y).conj() * c).real.sum()
+    got = torch.autograd.grad(loss, leaves)
+    assert seen[0].is_neg() and seen[0].size(1) == 1
+    want = torch.autograd.grad(DF.linear_act(x, w, b, act, r), leaves,
+                               seen[0].resolve_neg())
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    # the same of many outputs, contiguous
+    x, w, b = (torch.randn(*s, device=device, requires_grad=True)
+               for s in ((70, 24), (40, 24), (40,)))
+    dy = torch.randn(70, 40, device=device)
+    y = DF.linear_act(x, w, b, act)
+    want = torch.autograd.grad(y, (x, w, b), -dy, retain_graph=True)
+    got = torch.autograd.grad(y, (x, w, b), torch._neg_view(dy))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
