@@ -112,8 +112,8 @@ class AdamWPlan {
     });
   }
 
-  // Reads the gradients as they are now.  Those laid out unlike their
-  // parameter are copied into its layout first.  Returns the places (in this
+  // Reads the gradients as they are now.  Lazily negated ones, and those laid
+  // out unlike their parameter, are copied first.  Returns the places (in this
   // plan) of parameters with a gradient and no state.
   std::vector<int64_t> collect() {
     c10::DeviceGuard guard(device_);
@@ -126,8 +126,8 @@ class AdamWPlan {
       const State& s = states_[i];
       if (!s.step.defined()) missing.push_back(i);
       if (!s.step.defined() || p.numel() == 0) continue;
-      at::Tensor g = grad;
-      check_grad(g);
+      check_grad(grad);
+      at::Tensor g = grad.is_neg() ? grad.resolve_neg() : grad;
       TORCH_CHECK(p.device() == device_ && p.scalar_type() == dtype_ &&
                       same_layout(p, s.m),
                   "parameter ", indices_[i],

@@ -367,6 +367,9 @@ class FusedAdamW(torch.optim.Optimizer):
             if not _is_dense(p):
                 raise ValueError("a parameter is not dense in memory: the "
                                  "update runs over its storage")
+            if p.is_neg():
+                raise ValueError("a parameter is a lazy negation: the update "
+                                 "runs over its storage")
 
     # ---- state ------------------------------------------------------------
 

@@ -811,3 +811,27 @@ def test_8_bit_codes_of_spread_gradients_equal_the_cpu_path(dtype, offset):
         runs.append(state_of(opt, p))
     for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
         assert torch.equal(runs[0][k], runs[1][k]), k
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_lazily_negated_gradient(bits, device):
+    """A number that is the imaginary part of a conjugate gets one."""
+    a, b = (torch.nn.Parameter(torch.full((1,), 0.5, device=device))
+            for _ in range(2))
+    z = torch.complex(torch.zeros_like(a), a).conj()
+    (z * torch.tensor([1 + 2j], device=device)).real.sum().backward()
+    assert a.grad.is_neg() and float(a.grad) == 2.0
+    b.grad = torch.full_like(b, 2.0)
+    for p in (a, b):
+        FusedAdamW([p], lr=0.1, state_bits=bits, max_grad_norm=1.0).step()
+    assert torch.equal(a, b) and float(a) < 0.5
+    # the norm does not see the sign, and scaling keeps it
+    assert float(clip_grad_norm_([a], 1.0)) == 2.0
+    assert abs(float(a.grad) - 1.0) < 16 * U
+
+
+def test_lazily_negated_parameter_is_refused():
+    z = torch.zeros(1, dtype=torch.complex64).conj()
+    with pytest.raises(ValueError, match="negation"):
+        FusedAdamW([torch.nn.Parameter(z.imag)])
