@@ -519,7 +519,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def _build_plans(self):
         ext = load_kernels_ext()
         self._check_overlap()
-        self._plans = []
+        plans = []
         index = 0
         for group in self.param_groups:
             parts = {}
@@ -538,7 +538,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 plan = ext.AdamWPlan([p for _, p in members], *columns,
                                      [i for i, _ in members],
                                      group["state_bits"])
-                self._plans.append((plan, group, [p for _, p in members]))
+                plans.append((plan, group, [p for _, p in members]))
+        self._plans = plans
 
     def _step_gpu(self):
         if self._plans is None:

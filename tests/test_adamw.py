@@ -15,7 +15,8 @@ import pytest
 import torch
 from torch.optim.optimizer import register_optimizer_step_pre_hook
 
-from distributeddeeplearning_amd.ops import FusedAdamW, clip_grad_norm_
+from distributeddeeplearning_amd.ops import (FusedAdamW, clip_grad_norm_,
+                                             load_kernels_ext)
 from distributeddeeplearning_amd.ops import optim as O
 
 U = torch.finfo(torch.float32).eps / 2
@@ -835,3 +836,25 @@ def test_lazily_negated_parameter_is_refused():
     z = torch.zeros(1, dtype=torch.complex64).conj()
     with pytest.raises(ValueError, match="negation"):
         FusedAdamW([torch.nn.Parameter(z.imag)])
+
+
+@gpu
+def test_refused_step_is_refused_again():
+    """Nothing of a refused step is taken: no group of it, not later."""
+    p = make([30], torch.float32, "cuda") + make([30], torch.float32, "cpu")
+    before = [t.detach().clone() for t in p]
+    for groups in (p, [{"params": [p[0]]}, {"params": [p[1]]}]):
+        opt = FusedAdamW(groups)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="one optimizer"):
+                opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(p, before))
+
+
+def test_refused_plans_are_not_kept():
+    if load_kernels_ext(required=False) is None:
+        pytest.skip("extension not built")
+    opt = FusedAdamW(make([30], torch.float32, "cpu"))
+    with pytest.raises(ValueError, match="one optimizer"):
+        opt._build_plans()
+    assert opt._plans is None
