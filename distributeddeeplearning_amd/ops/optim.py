@@ -417,30 +417,71 @@ class FusedAdamW(torch.optim.Optimizer):
     def load_state_dict(self, sd):
         """Exact-dtype restore, as FusedSGD's; the state tensors of ``sd``
         are taken over without a copy where they are on the right device.
-        The state of a ``torch.optim.AdamW`` is understood too."""
-        for group in sd["param_groups"]:
+        The state of a ``torch.optim.AdamW`` is understood too.  A state that
+        is refused leaves the optimizer as it was."""
+        saved = sd["param_groups"]
+        if len(saved) != len(self.param_groups):
+            raise ValueError("loaded state dict has a different number of "
+                             "parameter groups")
+        options, owners = [], {}
+        for group, new in zip(self.param_groups, saved):
             for option in ("amsgrad", "maximize"):
-                if group.get(option):
+                if new.get(option):
                     raise ValueError(f"{option} is not supported")
-        _restore_exact(self, sd)
-        for group in self.param_groups:
-            group["betas"] = tuple(group["betas"])
-            for p in group["params"]:
-                self._adopt(p, self.state.get(p), group["state_bits"])
+            if len(group["params"]) != len(new["params"]):
+                raise ValueError("parameter group size mismatch in "
+                                 "load_state_dict")
+            ids = new["params"]
+            new = {**group, **new, "params": group["params"]}
+            new["betas"] = tuple(new["betas"])
+            self._check_group(new)
+            options.append(new)
+            for p, pid in zip(group["params"], ids):
+                owners[pid] = p, new["state_bits"]
+        state = {}
+        for pid, st in sd["state"].items():
+            if pid in owners:
+                p, bits = owners[pid]
+                state[p] = self._adopted(p, st, bits)
+            else:
+                state[pid] = dict(st)
+        for group, new in zip(self.param_groups, options):
+            group.update(new)
+        self.state.clear()
+        self.state.update(state)
         self._plans = None
 
     @staticmethod
-    def _adopt(p, st, bits):
+    def _adopted(p, st, bits):
+        """A loaded state entry as the optimizer holds it."""
+        st = {k: v.to(device=p.device) if torch.is_tensor(v) else v
+              for k, v in st.items()}
         if not st:
-            return
+            return st
+        names = ["exp_avg", "exp_avg_sq"]
+        scales = [name + "_scale" for name in names]
         if ("exp_avg_scale" in st) != (bits == 8):
             raise ValueError("the loaded moments and the group's state_bits "
                              "do not agree")
+        for name in names + (scales if bits == 8 else []) + ["step"]:
+            if name not in st:
+                raise ValueError(f"the loaded state has no {name}")
+        if bits == 8:
+            blocks = -(-p.numel() // MOMENT_BLOCK)
+            for name, scale in zip(names, scales):
+                if st[name].dtype != torch.uint8:
+                    raise ValueError(f"{name} holds uint8 codes, not "
+                                     f"{st[name].dtype}")
+                if st[scale].shape != (blocks,):
+                    raise ValueError(f"{scale} holds {blocks} scales")
+                st[scale] = st[scale].to(torch.float32).contiguous()
+        elif not all(st[name].is_floating_point() for name in names):
+            raise ValueError("moments of 32 bits are floating point")
         if p.dtype == torch.float32:
             st.pop("master", None)
         elif "master" not in st:
             st["master"] = p.detach().to(torch.float32)
-        for name in ("master", "exp_avg", "exp_avg_sq"):
+        for name in ["master"] + names:
             t = st.get(name)
             if t is None or _same_layout(t, p):
                 continue
@@ -450,13 +491,18 @@ class FusedAdamW(torch.optim.Optimizer):
             if bits == 8 and name != "master":
                 raise ValueError("8-bit moments belong to the memory layout "
                                  "that they were saved in")
-            st[name] = torch.empty_like(p, dtype=t.dtype).copy_(t)
-        if bits == 32:  # torch holds the moments in the parameter's dtype
-            for name in ("exp_avg", "exp_avg_sq"):
+            st[name] = torch.empty_like(
+                p, dtype=t.dtype, requires_grad=False).copy_(t)
+        # torch holds the moments in the parameter's dtype
+        for name in ["master"] + (names if bits == 32 else []):
+            if name in st:
                 st[name] = st[name].to(torch.float32)
         if not torch.is_tensor(st["step"]):
             st["step"] = torch.tensor(float(st["step"]))
+        if st["step"].numel() != 1:
+            raise ValueError("step holds one number")
         st["step"] = st["step"].to(p.device, torch.float32)
+        return st
 
     def __setstate__(self, state):
         super().__setstate__(state)

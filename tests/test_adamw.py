@@ -858,3 +858,72 @@ def test_refused_plans_are_not_kept():
     with pytest.raises(ValueError, match="one optimizer"):
         opt._build_plans()
     assert opt._plans is None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_refused_load_leaves_the_optimizer_as_it_was(bits, device):
+    """Every refusal concerns the last parameter or the last group: what was
+    looked at before it is not taken either."""
+    def build(state_bits=bits):
+        a = make([300, 5], torch.bfloat16, device)
+        b = make([70], torch.float32, device, seed=1)
+        opt = FusedAdamW([{"params": a}, {"params": b}], lr=1e-2,
+                         state_bits=state_bits)
+        opt.step()
+        return a + b, opt
+
+    params, opt = build()
+    twins, ref = build()
+
+    def kept(o):
+        return [(id(p), k, id(v)) for p, st in o.state.items()
+                for k, v in st.items()]
+
+    def change(fn, source=ref):
+        sd = copy.deepcopy(source.state_dict())
+        sd["param_groups"][0]["lr"] = 0.5
+        fn(sd)
+        return sd
+
+    last = 2
+    other = build(40 - bits)[1]
+    bad = [
+        change(lambda sd: sd["param_groups"][1].update(state_bits=40 - bits)),
+        change(lambda sd: None, other) | {
+            "param_groups": opt.state_dict()["param_groups"]},
+        change(lambda sd: sd["state"][last].update(
+            exp_avg=torch.zeros(71, dtype=sd["state"][last]["exp_avg"].dtype))),
+        change(lambda sd: sd["state"][last].pop("exp_avg_sq")),
+        change(lambda sd: sd["state"].update(
+            {last: {"momentum_buffer": torch.zeros(70)}})),
+        change(lambda sd: sd["state"][last].pop("step")),
+        change(lambda sd: sd["state"][last].update(step=torch.zeros(2))),
+        change(lambda sd: sd["param_groups"].pop()),
+        change(lambda sd: sd["param_groups"][1]["params"].append(3)),
+        change(lambda sd: sd["param_groups"][1].update(amsgrad=True)),
+        change(lambda sd: sd["param_groups"][1].update(betas=(0.9,))),
+    ]
+    if bits == 8:
+        bad += [
+            change(lambda sd: sd["state"][last].update(
+                exp_avg_sq_scale=torch.zeros(2))),
+            change(lambda sd: sd["state"][last].update(
+                exp_avg=torch.zeros(70))),
+        ]
+    else:
+        bad += [change(lambda sd: sd["state"][last].update(
+            exp_avg=torch.zeros(70, dtype=torch.uint8)))]
+    before, options = kept(opt), copy.deepcopy(opt.state_dict()["param_groups"])
+    for sd in bad:
+        saved = copy.deepcopy(sd)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(sd)
+        assert kept(opt) == before
+        assert opt.state_dict()["param_groups"] == options
+        assert str(sd) == str(saved)  # nor is what was offered
+    opt.step()
+    ref.step()
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q)
+        assert torch.equal(opt.state[p]["exp_avg"], ref.state[q]["exp_avg"])
