@@ -242,6 +242,37 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
         a.size(d) < 2 or a.stride(d) == b.stride(d) for d in range(a.dim()))
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Of two tensors whose address ranges overlap."""
+    if _is_dense(a) and _is_dense(b):
+        return True
+    if a.element_size() != b.element_size():
+        return True  # as far as can be told
+    places = []
+    for t in (a, b):
+        at = torch.tensor(t.data_ptr())
+        for size, stride in zip(t.shape, t.stride()):
+            at = at[..., None] + torch.arange(size) * (
+                stride * t.element_size())
+        places.append(at.flatten())
+    return bool(torch.isin(*places).any())
+
+
+def _shared_pair(tensors):
+    """Places of two tensors that share memory, or None."""
+    spans = sorted(
+        (str(t.device), t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
+            (size - 1) * stride for size, stride in zip(t.shape, t.stride()))),
+         i) for i, t in enumerate(tensors) if t.numel())
+    for k, (device, _, end, i) in enumerate(spans):
+        for other, start, _, j in spans[k + 1:]:
+            if other != device or start >= end:
+                break
+            if _share_memory(tensors[i], tensors[j]):
+                return min(i, j), max(i, j)
+    return None
+
+
 def _mix32(x: torch.Tensor) -> torch.Tensor:
     """The kernel's hash of 32 bits (held in int64)."""
     x = x ^ (x >> 16)
@@ -553,14 +584,10 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _check_overlap(self):
         """Tensors of one launch are updated at the same time."""
-        places = sorted(
-            (p.device.index, p.data_ptr(), p.numel() * p.element_size())
-            for g in self.param_groups for p in g["params"]
-            if p.is_cuda and p.numel()
-            and (p.grad is not None or p in self.state))
-        for (dev, at, size), (dev2, at2, _) in zip(places, places[1:]):
-            if dev == dev2 and at + size > at2:
-                raise ValueError("two parameters with gradients share memory")
+        if _shared_pair([p.detach() for g in self.param_groups
+                         for p in g["params"]
+                         if p.grad is not None or p in self.state]):
+            raise ValueError("two parameters with gradients share memory")
 
     def _build_plans(self):
         ext = load_kernels_ext()
@@ -614,6 +641,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def _step_cpu(self):
+        self._check_overlap()
         mul = 1.0 / self.grad_scale
         if self.max_grad_norm is not None:
             grads = [p.grad for g in self.param_groups for p in g["params"]
@@ -711,8 +739,9 @@ def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
         return load_kernels_ext().clip_grads(params, 1.0 / grad_scale,
                                              float(max_norm))
     grads = [p.grad for p in params if p.grad is not None]
-    if len({id(g) for g in grads}) != len(grads):
-        raise RuntimeError("a gradient appears twice")
+    if (len({id(g) for g in grads}) != len(grads)
+            or _shared_pair([g for g in grads if not g.is_sparse])):
+        raise RuntimeError("a gradient appears twice, or two share memory")
     norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
     if not float(coef) == 1.0:
         with torch.no_grad():

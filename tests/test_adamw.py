@@ -927,3 +927,39 @@ def test_refused_load_leaves_the_optimizer_as_it_was(bits, device):
     for p, q in zip(params, twins):
         assert torch.equal(p, q)
         assert torch.equal(opt.state[p]["exp_avg"], ref.state[q]["exp_avg"])
+
+
+def test_gradients_that_share_memory_are_refused_on_the_cpu():
+    a, b, c = make([4, 4, 4], torch.float32, "cpu")
+    base = torch.ones(9)
+    for first, second in ((base[:4], base[:4].view(4)), (base[:4], base[3:7]),
+                          (base[0:8:2], base[2:6]), (base[0:8:2], base[2:9:2])):
+        a.grad, b.grad = first, second
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip_grad_norm_([c, a, b], 1.0)
+        assert (base == 1).all()
+    # neighbours, and elements in turn, are apart
+    for first, second in ((base[:4], base[4:8]), (base[0:8:2], base[1:8:2])):
+        a.grad, b.grad = first, second
+        clip_grad_norm_([a, b], 0.5)
+        assert abs(float(base.norm()) - math.sqrt(1.25)) < 16 * U
+        base.fill_(1.0)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_that_share_memory_are_refused_on_the_cpu(bits):
+    base = torch.randn(100)
+    a, b, c = (torch.nn.Parameter(base[i:i + 50]) for i in (0, 49, 50))
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    before = base.clone()
+    for groups in ([a, b], [{"params": [b]}, {"params": [a], "lr": 0.1}]):
+        opt = FusedAdamW(groups, state_bits=bits)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share memory"):
+                opt.step()
+        assert torch.equal(base, before)
+    FusedAdamW([a, c], weight_decay=0.0, lr=0.5, state_bits=bits).step()
+    assert (base < before).all()
+    b.grad = None  # not updated
+    FusedAdamW([a, b, c], state_bits=bits).step()
