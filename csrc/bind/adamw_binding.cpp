@@ -103,6 +103,7 @@ class AdamWPlan {
       }
       states_.push_back(std::move(s));
     }
+    settle();
     // A launch takes so many tensors: the largest come first, so that all
     // launches but one are short.
     order_.resize(n);
@@ -118,6 +119,7 @@ class AdamWPlan {
   std::vector<int64_t> collect() {
     c10::DeviceGuard guard(device_);
     forget();
+    moved_ = false;
     std::vector<int64_t> missing;
     for (const int64_t i : order_) {
       const at::Tensor& p = params_[i];
@@ -150,6 +152,7 @@ class AdamWPlan {
       r.v = s.v.data_ptr();
       r.ms = bits_ == 8 ? s.ms.data_ptr<float>() : nullptr;
       r.vs = bits_ == 8 ? s.vs.data_ptr<float>() : nullptr;
+      if ((r.p ? r.p : r.w) != begins_[i]) moved_ = true;
       r.n = p.numel();
       r.step = s.step.data_ptr<float>();
       r.index = (uint32_t)indices_[i];
@@ -158,6 +161,15 @@ class AdamWPlan {
       grads_.push_back(std::move(g));
     }
     return missing;
+  }
+
+  // Whether collect() saw a parameter at another place in memory than
+  // settle() did, or the constructor.
+  bool moved() const { return moved_; }
+
+  void settle() {
+    begins_.clear();
+    for (const auto& p : params_) begins_.push_back(p.const_data_ptr());
   }
 
   std::vector<DdlGradTensor> grad_rows() const {
@@ -232,6 +244,8 @@ class AdamWPlan {
   at::ScalarType dtype_;
   std::vector<State> states_;
   std::vector<int64_t> order_;  // places, the largest parameter first
+  std::vector<const void*> begins_;  // of the parameters in memory
+  bool moved_ = false;
   std::vector<int64_t> places_;  // of what collect() saw, as are these
   std::vector<DdlAdamTensor> rows_;
   Tensors grads_;
@@ -353,7 +367,9 @@ void bind_adamw(pybind11::module& m) {
                           AdamWPlan::Maybe, AdamWPlan::Maybe, AdamWPlan::Maybe,
                           AdamWPlan::Maybe, AdamWPlan::Maybe,
                           std::vector<int64_t>, int64_t>())
-      .def("collect", &AdamWPlan::collect);
+      .def("collect", &AdamWPlan::collect)
+      .def("moved", &AdamWPlan::moved)
+      .def("settle", &AdamWPlan::settle);
   m.def("adamw_step", &adamw_step);
   m.def("clip_grads", &clip_grads);
 }

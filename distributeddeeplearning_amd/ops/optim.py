@@ -631,6 +631,10 @@ class FusedAdamW(torch.optim.Optimizer):
             self._build_plans()
             for plan, _, _ in self._plans:
                 plan.collect()
+        if any(plan.moved() for plan, _, _ in self._plans):
+            self._check_overlap()
+            for plan, _, _ in self._plans:
+                plan.settle()
         norm = load_kernels_ext().adamw_step(
             [plan for plan, _, _ in self._plans],
             [(g["lr"], *g["betas"], g["eps"], g["weight_decay"],

@@ -963,3 +963,27 @@ def test_parameters_that_share_memory_are_refused_on_the_cpu(bits):
     assert (base < before).all()
     b.grad = None  # not updated
     FusedAdamW([a, b, c], state_bits=bits).step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_parameters_moved_onto_one_another_are_refused(device):
+    """After a first step, too; apart again, they go on."""
+    a, b, c = make([50, 50, 3], torch.float32, device)
+    twins = make([50, 50, 3], torch.float32, device)
+    opt, ref = FusedAdamW([a, b, c]), FusedAdamW(twins)
+    opt.step()
+    ref.step()
+    kept = b.data
+    base = torch.zeros(99, device=device)
+    base[:50] = a.data
+    a.data = base[:50]
+    b.data = base[49:]
+    before = base.clone(), c.detach().clone()
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            opt.step()
+    assert torch.equal(base, before[0]) and torch.equal(c, before[1])
+    b.data = kept.clone()
+    opt.step()
+    ref.step()
+    assert all(torch.equal(p, q) for p, q in zip((a, b, c), twins))
