@@ -476,11 +476,26 @@ class FusedAdamW(torch.optim.Optimizer):
                 state[p] = self._adopted(p, st, bits)
             else:
                 state[pid] = dict(st)
+        self._part(state)
         for group, new in zip(self.param_groups, options):
             group.update(new)
         self.state.clear()
         self.state.update(state)
         self._plans = None
+
+    @staticmethod
+    def _part(state):
+        """Copies state tensors that share memory with others or with a
+        parameter: each is updated by itself, at the same time."""
+        owners = [(st, k) for p, st in state.items() if torch.is_tensor(p)
+                  for k, v in st.items() if torch.is_tensor(v)]
+        params = [p.detach() for p in state if torch.is_tensor(p)]
+        while True:
+            pair = _shared_pair(params + [st[k] for st, k in owners])
+            if pair is None or pair[1] < len(params):
+                return
+            st, k = owners[pair[1] - len(params)]
+            st[k] = st[k].clone()
 
     @staticmethod
     def _adopted(p, st, bits):

@@ -987,3 +987,48 @@ def test_parameters_moved_onto_one_another_are_refused(device):
     opt.step()
     ref.step()
     assert all(torch.equal(p, q) for p, q in zip((a, b, c), twins))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_loaded_state_tensors_that_share_memory_are_parted(bits, device):
+    """One step count for all parameters, one buffer of zeros for all
+    moments, as a program may write a state down."""
+    sizes = [300, 300, 20]
+    params, twins = (make(sizes, torch.float32, device) for _ in range(2))
+    kind = torch.uint8 if bits == 8 else torch.float32
+    opt, ref = (FusedAdamW(p, state_bits=bits) for p in (params, twins))
+    for o, shared in ((opt, True), (ref, False)):
+        sd = o.state_dict()
+        step = torch.full((), 5.0, device=device)
+        zeros = torch.zeros(300, dtype=kind, device=device)
+        scale = torch.ones(2, device=device)
+        for i, n in enumerate(sizes):
+            entry = {"step": step, "exp_avg": zeros[:n],
+                     "exp_avg_sq": zeros[:n]}
+            if bits == 8:
+                blocks = -(-n // 256)
+                entry.update(exp_avg_scale=scale[:blocks],
+                             exp_avg_sq_scale=scale[:blocks])
+            sd["state"][i] = {k: v if shared else v.clone()
+                              for k, v in entry.items()}
+        o.load_state_dict(sd)
+        for _ in range(2):
+            o.step()
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q)
+        a, b = state_of(opt, p), state_of(ref, q)
+        assert float(a["step"]) == 7
+        assert all(torch.equal(a[k], b[k]) for k in b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_loaded_state_is_taken_without_a_copy(device):
+    p, = make([300], torch.bfloat16, device)
+    opt = FusedAdamW([p])
+    opt.step()
+    sd = opt.state_dict()
+    again = FusedAdamW([p])
+    again.load_state_dict(sd)
+    for k, v in sd["state"][0].items():
+        assert again.state[p][k] is v
