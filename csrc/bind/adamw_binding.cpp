@@ -48,9 +48,16 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// False for a tensor whose storage was freed, and for autograd's zeros that
+// were never made: a kernel would read from address 0.
+bool has_memory(const at::Tensor& t) {
+  return t.numel() == 0 || t.storage().data() != nullptr;
+}
+
 void check_grad(const at::Tensor& g) {
   TORCH_CHECK(g.layout() == at::kStrided,
               "sparse gradients are not supported");
+  TORCH_CHECK(has_memory(g), "a gradient has no memory");
 }
 
 // The parameters of one group that share a device and a dtype, with their
@@ -134,6 +141,7 @@ class AdamWPlan {
                       same_layout(p, s.m),
                   "parameter ", indices_[i],
                   " changed its device, dtype, shape or layout");
+      TORCH_CHECK(has_memory(p), "parameter ", indices_[i], " has no memory");
       TORCH_CHECK(g.device() == device_ && g.scalar_type() == dtype_,
                   "the gradient of parameter ", indices_[i],
                   " differs from it in device or dtype");

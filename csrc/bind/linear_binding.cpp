@@ -34,6 +34,12 @@ int code_of(at::ScalarType t) {
   }
 }
 
+// False for a tensor whose storage was freed, and for autograd's zeros that
+// were never made: a kernel would read from address 0.
+bool has_memory(const at::Tensor& t) {
+  return t.numel() == 0 || t.storage().data() != nullptr;
+}
+
 constexpr int64_t LIMIT = (int64_t)1 << 29;
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -287,6 +293,9 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       if (want_x || want_w || want_b) {
+        for (const auto* t : {&dy, &saved[0], &saved[1], &saved[2]})
+          TORCH_CHECK_VALUE(!t->defined() || has_memory(*t),
+                            "a tensor of the backward pass has no memory");
         Grads g = backward_of(dy, saved[0], saved[1], saved[2],
                               ctx->saved_data["k"].toInt(),
                               ctx->saved_data["act"].toInt(), want_x, want_w,
@@ -333,6 +342,7 @@ at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w,
   auto plain = [&](const at::Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(!t.is_neg(), name, " is a lazy negation: call "
                       "resolve_neg() first");
+    TORCH_CHECK_VALUE(has_memory(t), name, " has no memory");
     TORCH_CHECK_NOT_IMPLEMENTED(!dual || !t._fw_grad(0).defined(), name,
                                 " carries a tangent: linear_act has no "
                                 "forward-mode derivative");

@@ -1032,3 +1032,26 @@ def test_loaded_state_is_taken_without_a_copy(device):
     again.load_state_dict(sd)
     for k, v in sd["state"][0].items():
         assert again.state[p][k] is v
+
+
+@gpu
+def test_tensors_without_memory_are_refused():
+    a, b = make([50, 60], torch.float32, "cuda")
+    opt = FusedAdamW([a, b])
+    opt.step()
+    before = a.detach().clone()
+    good, storage = b.grad, b.untyped_storage()
+    b.grad = torch.ones(70, device="cuda")[10:]
+    b.grad.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="gradient has no memory"):
+        opt.step()
+    with pytest.raises(RuntimeError, match="gradient has no memory"):
+        clip_grad_norm_([a, b], 1.0)
+    b.grad, size = good, storage.size()
+    storage.resize_(0)
+    with pytest.raises(RuntimeError, match="parameter 1 has no memory"):
+        opt.step()
+    assert torch.equal(a, before)
+    storage.resize_(size)
+    opt.step()
+    assert not torch.equal(a, before)

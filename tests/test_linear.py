@@ -659,3 +659,30 @@ def test_lazily_negated_gradient(act, device):
     want = torch.autograd.grad(y, (x, w, b), -dy, retain_graph=True)
     got = torch.autograd.grad(y, (x, w, b), torch._neg_view(dy))
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@gpu
+def test_tensors_without_memory_are_refused():
+    """A storage that was freed (also behind an offset), and zeros that were
+    never made."""
+    def freed(*shape):
+        t = torch.ones(2, *shape, device="cuda")[1]
+        t.untyped_storage().resize_(0)
+        return t
+
+    t = {"x": torch.randn(3, 8, device="cuda"),
+         "weight": torch.randn(5, 8, device="cuda"),
+         "bias": torch.randn(5, device="cuda"),
+         "residual": torch.randn(3, 5, device="cuda")}
+    for name, value in t.items():
+        for bad in (freed(*value.shape),
+                    torch._efficientzerotensor(value.shape, device="cuda")):
+            with pytest.raises(ValueError, match=f"{name} has no memory"):
+                DF.linear_act(**{**t, name: bad})
+    w = t["weight"].requires_grad_(True)
+    y = DF.linear_act(t["x"], w, None, "silu")
+    with pytest.raises(ValueError, match="no memory"):
+        torch.autograd.grad(y, w, freed(3, 5), retain_graph=True)
+    t["x"].untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="no memory"):
+        torch.autograd.grad(y, w, torch.ones_like(y))
