@@ -761,9 +761,16 @@ def clip_grad_norm_(params, max_norm, grad_scale=1.0) -> torch.Tensor:
     if (len({id(g) for g in grads}) != len(grads)
             or _shared_pair([g for g in grads if not g.is_sparse])):
         raise RuntimeError("a gradient appears twice, or two share memory")
+    for g in grads:
+        if g.device != first.device:
+            raise RuntimeError("all gradients are on one device")
+        if not g.is_floating_point():
+            raise RuntimeError(f"expected gradients of real numbers, got "
+                               f"{g.dtype}")
     norm, coef = _norm_cpu(grads, 1.0 / grad_scale, max_norm)
     if not float(coef) == 1.0:
         with torch.no_grad():
             for g in grads:
-                g.copy_(g.float() * coef)
+                wide = torch.promote_types(g.dtype, torch.float32)
+                g.copy_(g.to(wide) * coef)
     return norm

@@ -1055,3 +1055,23 @@ def test_tensors_without_memory_are_refused():
     storage.resize_(size)
     opt.step()
     assert not torch.equal(a, before)
+
+
+def test_clip_on_the_cpu_of_other_types():
+    """float64 keeps its bits: the scaling multiplies by one number, float32
+    of half a step; complex gradients are refused, not clipped by their real
+    parts."""
+    p = torch.nn.Parameter(torch.zeros(500, dtype=torch.float64))
+    torch.manual_seed(0)
+    p.grad = torch.randn(500, dtype=torch.float64)
+    before = p.grad.clone()
+    norm = clip_grad_norm_([p], 1.0)
+    assert abs(float(norm) / float(before.norm()) - 1) <= 2 * U
+    ratio = p.grad / before
+    assert float((ratio / ratio[0] - 1).abs().max()) < 1e-15
+    assert abs(float(ratio[0] * before.norm()) - 1) <= 8 * U + 1e-6
+    z = torch.nn.Parameter(torch.zeros(3, dtype=torch.complex64))
+    z.grad = torch.full((3,), 3j, dtype=torch.complex64)
+    with pytest.raises(RuntimeError, match="real numbers"):
+        clip_grad_norm_([p, z], 1.0)
+    assert (z.grad == 3j).all()
