@@ -198,9 +198,11 @@ __global__ __launch_bounds__(256) void act_bwd_k(
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void fold_bias_k(DdlBiasFold f) {
+__global__ __launch_bounds__(256) void fold_bias_k(DdlBiasFold f,
+                                                   int64_t first) {
   __shared__ __align__(16) char smem[256 * sizeof(double)];
-  fold_bias(f.partials, f.n, f.chunks, (T*)f.dbias, f.n, blockIdx.x, smem);
+  fold_bias(f.partials, f.n, f.chunks, (T*)f.dbias, f.n, first + blockIdx.x,
+            smem);
 }
 
 // ---- rows that do not begin at 4 bytes --------------------------------------
@@ -287,7 +289,8 @@ void ddl_backward_small(const DdlProduct* dx, const DdlProduct* dw,
 // 4096 10.9 (12.5), 1 x 2047 -> 1001 10.7 (13.6, of which packing 5), 1 x 4098
 // -> 4096 8.1 (11.8); float32, 16 x 14242 -> 2853 45 (71).
 bool ddl_few_rows_pay(const DdlProduct* p, bool aligned) {
-  if (p->m > 16 || p->n >= ((int64_t)1 << 26)) return false;  // its grid
+  // its grid: below 2^32 threads, 1024 of them for 16 outputs
+  if (p->m > 16 || cdiv(p->n, 16) >= ((int64_t)1 << 22)) return false;
   const float size = p->dtype == 0 ? 4.f : 2.f;
   const float row = p->r * size, all = row * p->n;
   float rate = 28e3f / (1.f + (p->dtype == 0 ? 0.4f : 0.8f) * p->m / 16.f);
@@ -327,11 +330,15 @@ void ddl_act_bwd(const void* dy, int64_t lddy, const void* z, int z_f32,
 }
 
 void ddl_fold_bias(const DdlBiasFold* f, int dtype, hipStream_t s) {
-  const unsigned blocks = (unsigned)cdiv(f->n, FOLD_COLS);
-  switch (dtype) {
-    case 0: fold_bias_k<float><<<blocks, 256, 0, s>>>(*f); break;
-    case 1: fold_bias_k<bf16><<<blocks, 256, 0, s>>>(*f); break;
-    case 2: fold_bias_k<f16><<<blocks, 256, 0, s>>>(*f); break;
+  const int64_t blocks = cdiv(f->n, FOLD_COLS);
+  constexpr int64_t MOST = (int64_t)1 << 23;  // a grid: below 2^32 threads
+  for (int64_t at = 0; at < blocks; at += MOST) {
+    const unsigned grid = (unsigned)std::min(MOST, blocks - at);
+    switch (dtype) {
+      case 0: fold_bias_k<float><<<grid, 256, 0, s>>>(*f, at); break;
+      case 1: fold_bias_k<bf16><<<grid, 256, 0, s>>>(*f, at); break;
+      case 2: fold_bias_k<f16><<<grid, 256, 0, s>>>(*f, at); break;
+    }
   }
 }
 

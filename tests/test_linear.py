@@ -686,3 +686,29 @@ def test_tensors_without_memory_are_refused():
     t["x"].untyped_storage().resize_(0)
     with pytest.raises(ValueError, match="no memory"):
         torch.autograd.grad(y, w, torch.ones_like(y))
+
+
+@gpu
+@pytest.mark.parametrize("n", [(1 << 26) - 16, (1 << 26) - 8, (1 << 26) + 8])
+def test_one_row_to_the_limits_of_a_grid(n):
+    w = torch.zeros(n, 8, dtype=torch.bfloat16, device="cuda")
+    w[::3] = 1.0
+    w[-1] = 2.0
+    x = torch.ones(1, 8, dtype=torch.bfloat16, device="cuda")
+    want = w[:, 0] * 8
+    assert torch.equal(DF.linear_act(x, w)[0], want)
+
+
+@gpu
+def test_bias_gradient_of_very_many_outputs():
+    n = (1 << 28) + 5
+    x = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda")
+    b = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    b.requires_grad_(True)
+    y = DF.linear_act(x, w, b)
+    assert (y == 1).all()
+    dy = (torch.arange(n, device="cuda", dtype=torch.int32) % 7).to(
+        torch.bfloat16)[None]
+    (db,) = torch.autograd.grad(y, b, dy)
+    assert torch.equal(db, dy[0])
