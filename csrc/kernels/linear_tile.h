@@ -71,21 +71,24 @@ struct Product {
 // ---- activations -----------------------------------------------------------
 
 // Functions of the activations.  FAST, for 16-bit types: the hardware's
-// reciprocal and power, off by one part in 2^22, and a fit of the normal
-// distribution, where float32 takes an IEEE division and erff.  GELU's backward
-// over 1024 x 4096 f16 takes 9.3 us so and 11.8 otherwise.
+// reciprocal and power, off by one part in 2^22 of themselves (the power's
+// argument is rounded besides, |z| 2^-24 of the result), and a fit of the normal
+// distribution, where float32 takes an IEEE division, expf and erff.  GELU's
+// backward over 1024 x 4096 f16 takes 9.3 us so and 11.8 with the latter two and
+// the hardware's power.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float z) {
   if constexpr (FAST)
     return __builtin_amdgcn_rcpf(
         1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
-  return 1.f / (1.f + __expf(-z));
+  return 1.f / (1.f + expf(-z));
 }
 
 // The standard normal distribution at z, and e = exp(-z^2 / 2).  FAST: below 0
-// it is e t P(t), t = 1 / (1 + 0.42 |z| / sqrt 2); P is a least-maximum fit of
-// exp(x^2) erfc(x) / 2t at x = |z| / sqrt 2.  Off by 1.7e-7, and in the tail by
-// 1.7e-5 of the value.
+// it is e t P(t), t = 1 / (1 + 0.42 |z| / sqrt 2), Hastings' form of the error
+// function (Abramowitz and Stegun 7.1.26); P, of degree 5, is a least-maximum fit
+// of exp(x^2) erfc(x) / 2t at x = |z| / sqrt 2, made for this kernel.  Off by
+// 1.7e-7, and in the tail by 1.7e-5 of the value.
 template <bool FAST>
 __device__ __forceinline__ float normal(float z, float& e) {
   if constexpr (FAST) {
@@ -100,7 +103,7 @@ __device__ __forceinline__ float normal(float z, float& e) {
     q *= t * e;
     return z < 0.f ? q : 1.f - q;
   }
-  e = __expf(-0.5f * z * z);
+  e = expf(-0.5f * z * z);
   return 0.5f * (1.f + erff(z * 0.70710678118654752f));
 }
 

@@ -712,3 +712,28 @@ def test_bias_gradient_of_very_many_outputs():
         torch.bfloat16)[None]
     (db,) = torch.autograd.grad(y, b, dy)
     assert torch.equal(db, dy[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_float32_tails_keep_their_bits(device):
+    """silu(z) = z / (1 + exp(-z)) in float32: exp good to 2 U of itself, the
+    sum, the quotient and the product to U each: 5 U of the value, also where
+    it is tiny; its derivative s (1 + z (1 - s)) below -4 to 4 U more, twice
+    that for 1 + z."""
+    z = torch.linspace(-80, 80, 4001, dtype=torch.float64).float()
+    for rows in (z[:, None], z[None, :]):  # tiled, and by few rows
+        one = torch.ones(1, 1, device=device)
+        x, w = (rows, one) if rows.size(1) == 1 else (one, rows.t())
+        x = x.to(device).requires_grad_(True)
+        w = w.to(device).contiguous().requires_grad_(True)
+        y = DF.linear_act(x, w, None, "silu")
+        d = z.double()
+        s = torch.sigmoid(d)
+        want = (d * s).reshape(y.shape)
+        check(y, want, 5 * U * want.abs() * (1 + 1e-6))
+        leaf = x if rows.size(1) == 1 else w
+        (g,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        slope = s * (1 + d * (1 - s))
+        tail = d < -4
+        check(g.flatten()[tail.to(device)], slope[tail],
+              13 * U * slope[tail].abs())
