@@ -737,3 +737,42 @@ def test_float32_tails_keep_their_bits(device):
         tail = d < -4
         check(g.flatten()[tail.to(device)], slope[tail],
               13 * U * slope[tail].abs())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("m", [12, 300])
+def test_backward_takes_z_as_it_was_summed(m, residual, act, dtype, device):
+    """Two rows whose z differ by less than a step of 16 bits, and whose dy
+    are 1 and -1: the bias gradient is the difference of two slopes, which z
+    rounded to the dtype would make zero.  Slopes are good to 16 U (|z| + 2)
+    and z to 4 U of its two terms' sizes, both below 2.01; db is summed before
+    dz is rounded, and rounded once."""
+    base = torch.tensor([0.5, -0.5, 1.0, -1.0, 2.0, -2.0])
+    near = 2.0 ** -13 if dtype == torch.float16 else 2.0 ** -10
+    x = torch.zeros(m, 2)
+    dy = torch.zeros(m, 6)
+    for c, z in enumerate(base.tolist()):
+        x[2 * c] = torch.tensor([z, z * near])
+        x[2 * c + 1] = torch.tensor([z, -z * near])
+        dy[2 * c, c], dy[2 * c + 1, c] = 1.0, -1.0
+    z = x.double().sum(1).requires_grad_(True)
+    assert torch.equal(x.to(dtype).float(), x)
+    if dtype != torch.float32:
+        assert torch.equal(z[:12].to(dtype), base.to(dtype).repeat_interleave(2))
+    (slope,) = torch.autograd.grad(act64(z, act).sum(), z)
+    want = slope[0:12:2] - slope[1:12:2]
+    x, w, b, dy = (t.to(device, dtype) for t in (
+        x, torch.ones(6, 2), torch.zeros(6), dy))
+    b.requires_grad_(True)
+    w.requires_grad_(True)
+    r = torch.zeros_like(dy) if residual else None
+    y = DF.linear_act(x, w, b, act, r)
+    db, _ = torch.autograd.grad(y, (b, w), dy)
+    room = 2 * (4 * U * 2.01 + 16 * U * 4.01) + 2 * U
+    # zero in its place would be found: it misses by |want|, and room and the
+    # rounding of db together are below 1.01 room + |want| / 256
+    assert float(want.abs().min()) > 2 * room
+    check(db, want, room + half(dtype) * (want.abs() + room))
