@@ -299,3 +299,57 @@ def test_two_ranks_agree(bits):
 def test_config_round_trips():
     cfg = _cfg(optimizer="adamw", clip_norm=1.0)
     assert TrainConfig(**dataclasses.asdict(cfg)) == cfg
+
+
+@pytest.mark.parametrize("device,dtype", [
+    ("cpu", torch.float32), pytest.param("cuda", torch.bfloat16, marks=gpu)])
+def test_fused_classifier_with_dropout(device, dtype):
+    """VGG's default of 0.5, the same masks: as without dropout, some roundings
+    of the dtype a layer, in float32 of 4096 and 25088 terms' sums."""
+    nets = [vgg16(num_classes=16, fused_classifier=f).classifier
+            for f in (False, True)]
+    nets[1].load_state_dict(nets[0].state_dict())
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(6, 25088, generator=gen).relu().to(device, dtype)
+    runs = []
+    for net in nets:
+        net = net.to(device)
+        ops.cast_model_(net, dtype)
+        assert net.training
+        torch.manual_seed(3)
+        ops.functional._DropoutFn._seed_counter[0] = 0
+        hidden = []
+        for part in (net[2], net[5]):
+            part.register_forward_hook(lambda _, __, y: hidden.append(y))
+        y = net(x)
+        y.float().square().sum().backward()
+        # about half of what the ReLU left open, of which about half
+        assert all(0.6 < float((h == 0).double().mean()) < 0.9 for h in hidden)
+        runs.append([y.detach()] + [p.grad for p in net.parameters()])
+    half = torch.finfo(dtype).eps / 2
+    room = 8 * half if dtype != torch.float32 else 64 * half
+    for a, b in zip(*runs):
+        a, b = a.double(), b.double()
+        assert (a - b).norm() <= room * a.norm()
+
+
+@gpu
+def test_trainer_with_fused_classifier():
+    """VGG-16 as it is trained: dropout, bfloat16, AdamW of 8 bits, clipping."""
+    tr = Trainer(_cfg(model="vgg16", image_size=224, dtype="bf16",
+                      device="cuda", optimizer="adamw", adam_state_bits=8,
+                      clip_norm=1.0, fused_classifier=True),
+                 steps_per_epoch=10)
+    assert [m.activation for m in tr.model.classifier
+            if isinstance(m, ops.Linear)] == ["relu", "relu", "none"]
+    assert [m.p for m in tr.model.classifier
+            if isinstance(m, ops.Dropout)] == [0.5, 0.5]
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    it = tr.data_iter()
+    for _ in range(2):
+        loss = tr.train_step(*next(it))
+        assert torch.isfinite(loss)
+        assert torch.isfinite(tr.opt.optimizer.grad_norm)
+    for p, q in zip(tr.model.parameters(), before):
+        assert not torch.equal(tr.opt.state[p]["master"], q.float())
+        assert torch.isfinite(p).all()
