@@ -346,7 +346,6 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     const int dtype = code_of(g.scalar_type());
     if (g.numel() == 0) continue;
     lists[dtype].rows.push_back(DdlGradTensor{g.data_ptr(), g.numel()});
-    written(g);
     const char* start = static_cast<const char*>(g.const_data_ptr());
     places.emplace_back(start, start + g.nbytes());
   }
@@ -364,6 +363,8 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     ddl_grad_scale(l.rows.data(), (int64_t)l.rows.size(), l.dtype, &norm.fold,
                    fold, stream_now());
   C10_HIP_KERNEL_LAUNCH_CHECK();
+  for (const auto& p : params)
+    if (p.grad().defined()) written(p.grad());
   return norm.norm;
 }
 

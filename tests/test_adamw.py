@@ -1075,3 +1075,17 @@ def test_clip_on_the_cpu_of_other_types():
     with pytest.raises(RuntimeError, match="real numbers"):
         clip_grad_norm_([p, z], 1.0)
     assert (z.grad == 3j).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refused_clipping_has_not_written(device):
+    a, b = make([5, 5], torch.float32, device)
+    versions = a.grad._version, b.grad._version
+    kept = a.grad, b.grad
+    b.grad = a.grad
+    with pytest.raises(RuntimeError, match="twice"):
+        clip_grad_norm_([a, b], 1e-3)
+    b.grad = kept[1]
+    assert (a.grad._version, b.grad._version) == versions
+    clip_grad_norm_([a, b], 1e-3)
+    assert a.grad._version > versions[0] and b.grad._version > versions[1]
