@@ -361,7 +361,7 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"max_grad_norm must be positive: {max_grad_norm}")
         self._plans = None
         super().__init__(params, defaults)
-        self.max_grad_norm = max_grad_norm
+        self.max_grad_norm = max_grad_norm  # None (later also 0): no clipping
         self.grad_scale = grad_scale  # multiply grads by 1/scale in the update
         self.grad_norm = None
 
@@ -590,6 +590,12 @@ class FusedAdamW(torch.optim.Optimizer):
 
     _hooked_step = torch.optim.Optimizer.profile_hook_step(_closure_step)
 
+    def _bound(self):
+        bound = self.max_grad_norm or 0.0
+        if not bound >= 0:
+            raise ValueError(f"max_grad_norm must be positive: {bound}")
+        return bound
+
     def _update(self):
         if self._plans is not None or any(
                 p.is_cuda for g in self.param_groups for p in g["params"]):
@@ -654,7 +660,7 @@ class FusedAdamW(torch.optim.Optimizer):
             [plan for plan, _, _ in self._plans],
             [(g["lr"], *g["betas"], g["eps"], g["weight_decay"],
               int(g["seed"]) & 0xFFFFFFFF) for _, g, _ in self._plans],
-            1.0 / self.grad_scale, self.max_grad_norm or 0.0)
+            1.0 / self.grad_scale, self._bound())
         if norm is not None:
             self.grad_norm = norm
 
@@ -662,7 +668,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step_cpu(self):
         self._check_overlap()
         mul = 1.0 / self.grad_scale
-        if self.max_grad_norm is not None:
+        if self._bound():
             grads = [p.grad for g in self.param_groups for p in g["params"]
                      if p.grad is not None]
             self.grad_norm, coef = _norm_cpu(grads, mul, self.max_grad_norm)

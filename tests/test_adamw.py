@@ -1089,3 +1089,23 @@ def test_refused_clipping_has_not_written(device):
     assert (a.grad._version, b.grad._version) == versions
     clip_grad_norm_([a, b], 1e-3)
     assert a.grad._version > versions[0] and b.grad._version > versions[1]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_bound_of_the_norm_changed_later(device):
+    a, b = make([50, 50], torch.float32, device)
+    b.data.copy_(a.data)
+    b.grad.copy_(a.grad)
+    opt, ref = FusedAdamW([a], max_grad_norm=1e-3), FusedAdamW([b])
+    opt.max_grad_norm = 0.0
+    opt.step()
+    ref.step()
+    assert torch.equal(a, b) and opt.grad_norm is None
+    for bad in (-1.0, float("nan")):
+        opt.max_grad_norm = bad
+        with pytest.raises(ValueError, match="positive"):
+            opt.step()
+    assert torch.equal(a, b) and float(opt.state[a]["step"]) == 1
+    opt.max_grad_norm = 1e-3
+    opt.step()
+    assert float(opt.grad_norm) > 1e-3
