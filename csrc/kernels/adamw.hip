@@ -276,7 +276,8 @@ __device__ __forceinline__ float half_wave_max(float x) {
 // Codes of 8 values of a lane, whose block's largest finite magnitude is
 // `top`.  An infinite or NaN value becomes a NaN code and leaves its block's
 // scale alone; a block whose values are all below 2^-100 becomes zeros.
-// LEAST: a positive value of another block takes at least the smallest code.
+// LEAST: no value is below zero, and a positive one of another block takes at
+// least the smallest code.
 template <bool LEAST>
 __device__ __forceinline__ uint2 encode8(const float* x, float top,
                                          const uint32_t* r, int shift,
@@ -288,9 +289,9 @@ __device__ __forceinline__ uint2 encode8(const float* x, float top,
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float y = fminf(fabsf(x[j]) * inv, 448.f);
-    float code = round_by_chance(y, (r[j] >> shift) & 0xFFFFu);
-    if (LEAST && y > 0.f) code = fmaxf(code, 0x1p-9f);
-    const float e = copysignf(code, x[j]);
+    const float code = round_by_chance(y, (r[j] >> shift) & 0xFFFFu);
+    const float e = LEAST ? fmaxf(code, y > 0.f ? 0x1p-9f : 0.f)
+                          : copysignf(code, x[j]);
     q[j] = finite(x[j]) ? e : __uint_as_float(0x7FC00000u);
   }
   return uint2{pack4(q), pack4(q + 4)};
