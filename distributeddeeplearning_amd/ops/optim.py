@@ -14,6 +14,8 @@ and biases) as required by the batch-8k config (BASELINE.json:9).
 """
 from __future__ import annotations
 
+import itertools
+
 import torch
 from torch.optim.optimizer import (_global_optimizer_post_hooks,
                                    _global_optimizer_pre_hooks)
@@ -258,15 +260,22 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return bool(torch.isin(*places).any())
 
 
+def _bytes(t: torch.Tensor) -> int:
+    """From a tensor's first element to its last one's end."""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    return t.element_size() * (1 + sum(
+        (size - 1) * stride for size, stride in zip(t.shape, t.stride())))
+
+
 def _shared_pair(tensors):
     """Places of two tensors that share memory, or None."""
-    spans = sorted(
-        (str(t.device), t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
-            (size - 1) * stride for size, stride in zip(t.shape, t.stride()))),
-         i) for i, t in enumerate(tensors) if t.numel())
-    for k, (device, _, end, i) in enumerate(spans):
-        for other, start, _, j in spans[k + 1:]:
-            if other != device or start >= end:
+    spans = [(t.get_device(), t.data_ptr(), _bytes(t), i)
+             for i, t in enumerate(tensors) if t.numel()]
+    spans.sort()
+    for k, (device, at, size, i) in enumerate(spans):
+        for other, start, _, j in itertools.islice(spans, k + 1, None):
+            if other != device or start >= at + size:
                 break
             if _share_memory(tensors[i], tensors[j]):
                 return min(i, j), max(i, j)
@@ -605,8 +614,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _check_overlap(self):
         """Tensors of one launch are updated at the same time."""
-        if _shared_pair([p.detach() for g in self.param_groups
-                         for p in g["params"]
+        if _shared_pair([p for g in self.param_groups for p in g["params"]
                          if p.grad is not None or p in self.state]):
             raise ValueError("two parameters with gradients share memory")
 
