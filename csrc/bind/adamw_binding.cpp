@@ -334,6 +334,8 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
   for (int i = 0; i < 3; ++i) lists[i].dtype = i;
   std::vector<std::pair<const char*, const char*>> places;
   places.reserve(params.size());
+  std::vector<const at::Tensor*> grads;
+  grads.reserve(params.size());
   c10::optional<c10::Device> device;
   for (const auto& p : params) {
     const at::Tensor& g = p.grad();
@@ -346,6 +348,7 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     const int dtype = code_of(g.scalar_type());
     if (g.numel() == 0) continue;
     lists[dtype].rows.push_back(DdlGradTensor{g.data_ptr(), g.numel()});
+    grads.push_back(&g);
     const char* start = static_cast<const char*>(g.const_data_ptr());
     places.emplace_back(start, start + g.nbytes());
   }
@@ -363,8 +366,7 @@ at::Tensor clip_grads(const std::vector<at::Tensor>& params, double grad_mul,
     ddl_grad_scale(l.rows.data(), (int64_t)l.rows.size(), l.dtype, &norm.fold,
                    fold, stream_now());
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  for (const auto& p : params)
-    if (p.grad().defined()) written(p.grad());
+  for (const at::Tensor* g : grads) written(*g);
   return norm.norm;
 }
 
