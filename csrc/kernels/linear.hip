@@ -113,7 +113,8 @@ void run_few(const DdlProduct* p, hipStream_t s) {
 // ---- backward of the activation, bias gradient ------------------------------
 
 // 256 threads take 8 columns each: LANES of them a row, all rows of a turn
-// twice.  64 columns a block where there are no more, 256 otherwise.
+// twice.  64 columns a block where there are no more, 256 otherwise.  A block
+// adds its rows of a column in float32, the fold adds the blocks in 64 bits.
 constexpr int BWD_NARROW = 8, BWD_WIDE = 32;
 
 // Rows that a block sums: one turn where there are few, as many turns as leave
