@@ -15,8 +15,7 @@ import pytest
 import torch
 from torch.optim.optimizer import register_optimizer_step_pre_hook
 
-from distributeddeeplearning_amd.ops import (FusedAdamW, clip_grad_norm_,
-                                             load_kernels_ext)
+from distributeddeeplearning_amd.ops import FusedAdamW, clip_grad_norm_
 from distributeddeeplearning_amd.ops import optim as O
 
 U = torch.finfo(torch.float32).eps / 2
@@ -852,7 +851,7 @@ def test_refused_step_is_refused_again():
 
 
 def test_refused_plans_are_not_kept():
-    if load_kernels_ext(required=False) is None:
+    if O.load_kernels_ext(required=False) is None:
         pytest.skip("extension not built")
     opt = FusedAdamW(make([30], torch.float32, "cpu"))
     with pytest.raises(ValueError, match="one optimizer"):
